@@ -478,9 +478,9 @@ struct LateAcc {
 #define FA_HALF_BF16_PACKED 1
 #endif
 #if FA_HALF_BF16_PACKED
-// bfloat16: the same operations on PAIRS of elements, so that the three fp32 operations of a
-// client's term are packed instructions (v_pk_add_f32 / v_pk_mul_f32: two elements each); every
-// result is still rounded on its own (one conversion per element).
+// bfloat16: the same operations on PAIRS of elements, as the 16-bit loads bring them (the library is
+// built without packed fp32 instructions, so each operation of a pair is one instruction per
+// element); every result is still rounded on its own (one conversion per element).
 template <>
 struct LateAcc<FA_HALF_BF16> {
     f2 g[4], s[4];
