@@ -37,6 +37,32 @@ class MeanSegment(C.Structure):
     _fields_ = [("row_offset", C.c_size_t), ("out", C.c_void_p), ("n", C.c_size_t),
                 ("dtype", C.c_int)]
 
+
+FA_LOGITS_F32, FA_LOGITS_BF16, FA_LOGITS_F16 = range(3)
+FA_TOP_MAX, FA_MERGE_CLIENTS, FA_MERGE_ENTRIES = 256, 128, 8192
+
+
+class Logits(C.Structure):
+    """``fa_logits``: rows of logits (token operators)."""
+    _fields_ = [("data", C.c_void_p), ("outer", C.c_int64), ("inner", C.c_int64),
+                ("stride_outer", C.c_int64), ("stride_inner", C.c_int64), ("vocab", C.c_int),
+                ("dtype", C.c_int)]
+
+
+class Teacher(C.Structure):
+    """``fa_teacher``: one list of tokens per row (distillation)."""
+    _fields_ = [("ids", C.c_void_p), ("logprobs", C.c_void_p), ("id_stride", C.c_int64),
+                ("lp_stride", C.c_int64), ("row_weight", C.c_void_p), ("temperature", C.c_double),
+                ("k", C.c_int)]
+
+
+class Tops(C.Structure):
+    """``fa_tops``: the clients' lists (fa_merge_tops)."""
+    _fields_ = [("ids", C.c_void_p), ("logprobs", C.c_void_p), ("id_client", C.c_int64),
+                ("id_row", C.c_int64), ("lp_client", C.c_int64), ("lp_row", C.c_int64),
+                ("token_weight", C.c_void_p), ("unit_client", C.c_int64), ("unit_row", C.c_int64),
+                ("k", C.c_int)]
+
 # name -> (restype, argtypes); mirrors include/appfl_amd.h one to one.
 SIGNATURES = {
     "fa_version": (_i, []),
@@ -104,6 +130,12 @@ SIGNATURES = {
     "fa_half_buff_flush_mean": (_i, [_p, _p, _i, _sz, _i, _p]),
     "fa_half_fill": (_i, [_p, _d, _sz, _i, _p]),
     "fa_synth_fill": (_i, [_p, _p, _sz, _u64, _u64, _f, _p]),
+    "fa_token_workspace": (_i, [_p, _i, _p]),
+    "fa_token_scores": (_i, [_p, _p, C.c_int64, _i, _p, _p, _p, _p, _p, _p, _p]),
+    "fa_merge_tops": (_i, [_p, _p, _i, C.c_int64, _i, _p, _p, _p]),
+    "fa_distill_loss": (_i, [_p, _p, _p, _p, _p, _p]),
+    "fa_distill_grad": (_i, [_p, _p, _p, _p, _p, C.c_int64, C.c_int64, _p]),
+    "fa_distill_loss_grad": (_i, [_p, _p, _p, _p, C.c_int64, C.c_int64, _p, _p]),
     "fa_pack_host": (_i, [_p, _p, _p, _p, _i, _i]),
     "fa_pack_host_window": (_i, [_p, _p, _p, _p, _i, _sz, _sz, _i]),
     "fa_host_copy_fresh": (_i, [_p, _p, _sz, _i]),

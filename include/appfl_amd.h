@@ -484,6 +484,100 @@ int fa_synth_fill(float* p, const float* base, size_t n, uint64_t seed, uint64_t
                   float scale, fa_stream_t stream);
 
 /*
+ * Operators on ANSWERS, for federations whose clients exchange what their models answer on a public
+ * set instead of the models' weights (aggregation by distillation; no counterpart in the reference,
+ * whose aggregators average weights).  A position's answer is a list of its most probable tokens
+ * (or classes) with their log probabilities, best first.  Shared rules:
+ *   - logits are fp32, bfloat16 or float16 rows of `vocab` adjacent elements, found at
+ *     data + (o * stride_outer + i * stride_inner) elements for o < outer, i < inner (a
+ *     [batch, sequence, vocab] view such as logits[:, :-1], or inner = rows, outer = 1); any row
+ *     may start at any element.  outer * inner < 2^31.
+ *   - list entries with a negative id are absent; ids are int32, log probabilities fp32.
+ *   - softmax statistics and sums are fp32, merged probabilities fp64.
+ *   - per-row results are written in row order, packed.
+ */
+enum { FA_LOGITS_F32 = 0, FA_LOGITS_BF16 = 1, FA_LOGITS_F16 = 2 };
+#define FA_TOP_MAX 256         /* entries of one list                                         */
+#define FA_MERGE_CLIENTS 128   /* clients of one fa_merge_tops call                           */
+#define FA_MERGE_ENTRIES 8192  /* clients * entries of one list of one fa_merge_tops call     */
+
+typedef struct {
+    const void* data;
+    int64_t outer, inner, stride_outer, stride_inner;
+    int vocab;
+    int dtype;               /* FA_LOGITS_* */
+} fa_logits;
+
+typedef struct {             /* one list per row: entry j of row r at ids[r * id_stride + j] */
+    const int32_t* ids;
+    const float* logprobs;
+    int64_t id_stride, lp_stride;
+    const float* row_weight; /* one per row, packed; NULL: 1 */
+    double temperature;      /* in [1e-30, 1e30] */
+    int k;                   /* 1..FA_TOP_MAX */
+} fa_teacher;
+
+typedef struct {             /* entry j of client c's row r at ids[c * id_client + r * id_row + j] */
+    const int32_t* ids;
+    const float* logprobs;
+    int64_t id_client, id_row, lp_client, lp_row;
+    const float* token_weight;  /* [c * unit_client + r * unit_row]; NULL: 1 */
+    int64_t unit_client, unit_row;
+    int k;                      /* 1..FA_TOP_MAX */
+} fa_tops;
+
+/* *bytes = size of the device workspace `ws` that the calls below need for these logits and `top`
+ * (fa_token_scores; 0 for the distillation calls); 0: ws may be NULL.  Depends on the current
+ * device's size.  A workspace belongs to one call at a time. */
+int fa_token_workspace(const fa_logits* logits, int top, size_t* bytes);
+
+/*
+ * Per row:  lse = log sum_v exp x_v;  entropy = sum_v p_v (lse - x_v), p = exp(x - lse);
+ *   logprob = x_target - lse (0 where target == ignore_index, NaN where it is outside the
+ *   vocabulary);  top_ids / top_logprobs: the `top` largest logits, best first, equal ones (and -0
+ *   and +0) by the lower id first, NaN before everything.
+ * A row of nothing but -inf has lse = -inf, entropy 0 and log probabilities of -inf.  targets and
+ * logprob may both be NULL; 0 <= top <= min(vocab, FA_TOP_MAX).
+ */
+int fa_token_scores(const fa_logits* logits, const int64_t* targets, int64_t ignore_index, int top,
+                    float* logprob, float* entropy, float* lse, int32_t* top_ids,
+                    float* top_logprobs, void* ws, fa_stream_t stream);
+
+/*
+ * Weighted mean of K clients' answers, cut to its `top` largest entries:
+ *   p(v) = sum_c w_c u_c exp(lp_c(v)) / sum_{c answering} w_c u_c
+ * in fp64, clients in order c = 0..K-1, entries of one client in list order (an id listed twice
+ * counts twice).  w: HOST array of K finite weights >= 0; u: token_weight.  A client whose w_c u_c
+ * is not above zero, or whose list is empty, does not answer that row.  Output best first, equal
+ * values by the lower id first; id -1 and -inf where a row has fewer than `top` different tokens.
+ * 1 <= top <= K * k.
+ */
+int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int top, int32_t* out_ids,
+                  float* out_logprobs, fa_stream_t stream);
+
+/*
+ * Distillation from a teacher's list.  With t = softmax over the list's entries of lp / T and
+ * q = softmax over the vocabulary of x / T, per row
+ *   loss = weight * T^2 * sum_j t_j (log t_j - log q[id_j])
+ *   d loss / d x_v = weight * T * (q_v - sum_{j: id_j = v} t_j)
+ * fa_distill_loss writes the losses and, for the backward call, `stat` (2 floats per row);
+ * fa_distill_grad writes the gradient of sum_r row_grad[r] * loss[r] (row_grad NULL: 1);
+ * fa_distill_loss_grad does both (row_grad 1) and may write the gradient over the logits (same
+ * data and strides).  The gradient has the logits' type and row shape, with strides of its own;
+ * its rows must not overlap.  A row with weight 0 or without an entry of probability above 0 has
+ * loss and gradient 0 whatever its logits hold; an id >= vocab makes its row's loss and gradient
+ * NaN.  A logit of -inf has q = 0 (loss inf where the teacher wants it).
+ */
+int fa_distill_loss(const fa_logits* logits, const fa_teacher* teacher, float* loss, float* stat,
+                    void* ws, fa_stream_t stream);
+int fa_distill_grad(const fa_logits* logits, const fa_teacher* teacher, const float* stat,
+                    const float* row_grad, void* grad, int64_t grad_stride_outer,
+                    int64_t grad_stride_inner, fa_stream_t stream);
+int fa_distill_loss_grad(const fa_logits* logits, const fa_teacher* teacher, float* loss, void* grad,
+                         int64_t grad_stride_outer, int64_t grad_stride_inner, void* ws,
+                         fa_stream_t stream);
+
+/*
  * Host-side packing of one client's state dict into a row of a (pinned) staging slab:
  * for t in 0..T-1: memcpy(dst + dst_off[t], src[t], nbytes[t]), spread over `threads` threads.
  * All pointers are HOST memory.  Stands where the reference materialises per-tensor CPU
