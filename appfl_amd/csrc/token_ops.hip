@@ -17,6 +17,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWave = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kInf = __builtin_inff();
 
 using u16 = unsigned short;
@@ -50,66 +51,194 @@ struct Rows {            // a [outer, inner, vocab] view with unit stride along 
     }
 };
 
-// ---- softmax statistics: m = max x, s = sum exp((x - m) / tau), e = sum exp((x - m) / tau) (x - m) / tau
-struct Stat {
-    float m, s, e;
+// 16 bytes of a row, and the rest of it: `head` elements before the first 16-byte boundary, `nvec`
+// vectors, `tail` elements behind the last one.
+struct Span {
+    int head, nvec, tail;
 };
 
-__device__ __forceinline__ Stat stat_empty() { return {-kInf, 0.0f, 0.0f}; }
+template <int DT>
+struct Vec {
+    using Raw = typename Elem<DT>::Raw;
+    static constexpr int N = 16 / sizeof(Raw);
+    // what fills the lanes past the end of a row
+    static constexpr unsigned kFill = DT == FA_LOGITS_F32 ? 0xff800000u : DT == FA_LOGITS_BF16 ? 0xff80ff80u : 0xfc00fc00u;
 
-// exp2 of the hardware: below 2^-126 it returns 0, which is nothing beside the largest term's 1
-__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+    static __device__ __forceinline__ Span span(const Raw* x, int vocab) {
+        const unsigned off = static_cast<unsigned>(reinterpret_cast<uintptr_t>(x)) % 16 / sizeof(Raw);
+        Span s;
+        s.head = off ? N - static_cast<int>(off) : 0;
+        if (s.head > vocab) s.head = vocab;
+        s.nvec = (vocab - s.head) / N;
+        s.tail = vocab - s.head - s.nvec * N;
+        return s;
+    }
+    static __device__ __forceinline__ uint4 fill() { return {kFill, kFill, kFill, kFill}; }
+    static __device__ __forceinline__ void widen(const uint4& r, float (&v)[N]) {
+        const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == FA_LOGITS_F32) {
+                v[i] = __uint_as_float(w[i]);
+            } else if constexpr (DT == FA_LOGITS_BF16) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            } else {
+                v[2 * i] = Elem<DT>::widen(static_cast<u16>(w[i]));
+                v[2 * i + 1] = Elem<DT>::widen(static_cast<u16>(w[i] >> 16));
+            }
+        }
+    }
+    static __device__ __forceinline__ uint4 narrow(const float (&v)[N]) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == FA_LOGITS_F32)
+                w[i] = __float_as_uint(v[i]);
+            else
+                w[i] = Elem<DT>::narrow(v[2 * i]) | static_cast<unsigned>(Elem<DT>::narrow(v[2 * i + 1])) << 16;
+        }
+        return {w[0], w[1], w[2], w[3]};
+    }
+};
 
-// Two parts of a row.  A part without a finite logit has s = 0 and adds nothing; a NaN stays a NaN.
-__device__ __forceinline__ Stat stat_join(const Stat a, const Stat b, float scale2) {
-    Stat r;
-    r.m = fmaxf(a.m, b.m);
-    const float ref = r.m == -kInf ? 0.0f : r.m;
-    const float da = (a.m - ref) * scale2, db = (b.m - ref) * scale2;     // log2 units
-    const float fa = exp2_hw(da), fb = exp2_hw(db);
-    // a part too far below (its distance may be -inf) or without a finite logit adds nothing
-    const float ea = a.s == 0.0f || fa == 0.0f ? 0.0f : fa * (a.e + a.s * da);
-    const float eb = b.s == 0.0f || fb == 0.0f ? 0.0f : fb * (b.e + b.s * db);
-    r.s = a.s * fa + b.s * fb;
-    r.e = ea + eb;
-    return r;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// A row that is read once: past the caches.
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    return {v.x, v.y, v.z, v.w};
 }
 
-__device__ __forceinline__ Stat stat_wave(Stat v, float scale2) {
+// ---- softmax statistics ---------------------------------------------------------------------------
+// With k = log2(e) / T every term is 2^(x k - R), R a whole number near the largest x k: the
+// multiply-add rounds once, relative to its small result, rescaling by a power of two is exact, and
+// the rounding of k is a change of T by 2^-25 that all of a row's terms share.
+//   s = sum 2^(x k - R),   e = sum 2^(x k - R) (x k - R)   (entropy = (log2 s - e / s) / k)
+// R stays within +-kFar, so a distance is finite; a row whose x k lies beyond (a row of the type's
+// lowest value, infinities) or holds a NaN ends with s = 0, inf or NaN and is taken again by
+// slow_stat, which subtracts the maximum before it scales.
+constexpr float kFar = 1e38f;
+
+struct Acc {
+    float R, s, e;
+};
+
+__device__ __forceinline__ Acc acc_empty() { return {-kFar, 0.0f, 0.0f}; }
+
+// exp2 of the hardware: below 2^-126 it returns 0, which is nothing beside the largest term
+__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+template <bool ENT>
+__device__ __forceinline__ void acc_raise(Acc& a, float R) {
+    const float d = a.R - R, f = exp2_hw(d);
+    if (ENT) a.e = f * (a.e + a.s * d);
+    a.s *= f;
+    a.R = R;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void acc_one(Acc& a, float v, float k) {
+    const float y = fmaf(v, k, -a.R);
+    const float t = exp2_hw(y);
+    a.s += t;
+    if (ENT) a.e = fmaf(t, fmaxf(y, -200.0f), a.e);       // 0 * -inf; a NaN stays in t
+}
+
+// N terms whose largest is `top`
+template <bool ENT, int N>
+__device__ __forceinline__ void acc_add(Acc& a, const float (&v)[N], float top, float k) {
+    acc_raise<ENT>(a, fmaxf(a.R, fminf(rintf(top * k), kFar)));
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc_one<ENT>(a, v[i], k);
+}
+
+template <bool ENT>
+__device__ __forceinline__ Acc acc_join(Acc a, Acc b) {
+    const float R = fmaxf(a.R, b.R);
+    acc_raise<ENT>(a, R);
+    acc_raise<ENT>(b, R);
+    return {R, a.s + b.s, a.e + b.e};
+}
+
+template <bool ENT>
+__device__ __forceinline__ Acc acc_wave(Acc v) {
+#pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) {
-        Stat o;
-        o.m = __shfl_xor(v.m, d);
+        Acc o;
+        o.R = __shfl_xor(v.R, d);
         o.s = __shfl_xor(v.s, d);
-        o.e = __shfl_xor(v.e, d);
-        v = stat_join(v, o, scale2);
+        o.e = ENT ? __shfl_xor(v.e, d) : 0.0f;
+        v = acc_join<ENT>(v, o);
     }
     return v;
 }
 
-template <int THREADS>
-__device__ __forceinline__ Stat stat_block(Stat v, float scale2, Stat* lds) {
-    v = stat_wave(v, scale2);
+// Ends with every thread holding the row's sums; one barrier, `lds` is not used again in the row.
+template <bool ENT, int THREADS>
+__device__ __forceinline__ Acc acc_block(Acc v, Acc* lds) {
+    v = acc_wave<ENT>(v);
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
     __syncthreads();
-    Stat r = lds[0];
-    for (int i = 1; i < THREADS / kWave; ++i) r = stat_join(r, lds[i], scale2);
-    __syncthreads();
+    Acc r = lds[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / kWave; ++i) r = acc_join<ENT>(r, lds[i]);
     return r;
 }
 
-// e is kept in log2 units: entropy = log s - e ln 2 / s
-constexpr float kLn2 = 0.69314718055994530942f;
+// What a row's softmax is afterwards.  slow: in terms of m and log s (natural, of (x - m) / T).
+struct RowStat {
+    float R, s, m, log_s, entropy;
+    bool slow;
+};
 
-template <int DT>
-__device__ __forceinline__ Stat row_stat(const typename Elem<DT>::Raw* x, int vocab, float scale2, Stat* lds) {
-    Stat st = stat_empty();
-    for (int i = threadIdx.x; i < vocab; i += kThreads) {
-        const float v = Elem<DT>::widen(x[i]);
-        const Stat one = {v, v == -kInf ? 0.0f : (v != v ? v : 1.0f), 0.0f};
-        st = stat_join(st, one, scale2);
-    }
-    return stat_block<kThreads>(st, scale2, lds);
+template <int THREADS>
+__device__ float block_max_f(float v, float* lds) {
+    for (int d = kWave / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+    float r = lds[0];
+    for (int i = 1; i < THREADS / kWave; ++i) r = fmaxf(r, lds[i]);
+    return r;
 }
+
+template <int THREADS>
+__device__ float block_sum_f(float v, float* lds) {
+    for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+    float r = lds[0];
+    for (int i = 1; i < THREADS / kWave; ++i) r += lds[i];
+    return r;
+}
+
+// Rows the fast sums cannot hold: two plain passes.  A row of nothing but -inf has s = 0.
+template <int DT, int THREADS>
+__device__ __attribute__((noinline)) RowStat slow_stat(const typename Elem<DT>::Raw* x, int vocab, float inv_tau, float* lds) {
+    float m = -kInf;
+    for (int i = threadIdx.x; i < vocab; i += THREADS) m = fmaxf(m, Elem<DT>::widen(x[i]));
+    m = block_max_f<THREADS>(m, lds);
+    const float ref = m == -kInf ? 0.0f : m;
+    float s = 0.0f, e = 0.0f;
+    for (int i = threadIdx.x; i < vocab; i += THREADS) {
+        const float d = (Elem<DT>::widen(x[i]) - ref) * inv_tau, t = exp2_hw(d * kLog2e);
+        s += t;
+        if (t != 0.0f) e += t * d;
+    }
+    s = block_sum_f<THREADS>(s, lds);
+    e = block_sum_f<THREADS>(e, lds);
+    RowStat r = {0.0f, s, m, logf(s), 0.0f, true};
+    r.entropy = s == 0.0f ? 0.0f : r.log_s - e / s;
+    return r;
+}
+
+__device__ __forceinline__ bool acc_good(const Acc& a) { return a.s > 0.0f && a.s < kInf; }
+
+struct Scale {               // k = fl(log2(e) / T), 1 / k, 1 / T
+    float k, inv_k, inv_tau;
+};
 
 // ---- order of logits: by value, ties to the lowest index, NaN first; -0 and +0 are equal ----------
 __device__ __forceinline__ uint64_t order_key(float v, unsigned index) {
@@ -119,22 +248,141 @@ __device__ __forceinline__ uint64_t order_key(float v, unsigned index) {
     return (static_cast<uint64_t>(o) << 32) | (0xffffffffu - index);
 }
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-    for (int d = kWave / 2; d > 0; d >>= 1) {
-        const uint64_t o = __shfl_xor(static_cast<unsigned long long>(v), d);
-        v = o > v ? o : v;
-    }
-    return v;
+__device__ __forceinline__ unsigned key_index(uint64_t key) { return 0xffffffffu - static_cast<unsigned>(key); }
+
+__device__ __forceinline__ float key_value(uint64_t key) {       // not for a NaN's key
+    const unsigned o = static_cast<unsigned>(key >> 32);
+    return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, uint64_t* lds) {
-    v = wave_max_u64(v);
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+// ---- the top entries of a row ---------------------------------------------------------------------
+// One pass.  The row is read in chunks of adjacent elements.  From the first chunk every thread
+// contributes its largest key; the top-th largest of those is a bound that at least `top` elements
+// reach, and the elements that reach it become candidates.  From then on only elements above the
+// current top-th value are candidates (an equal one has a higher index), found by comparing the
+// largest of a thread's elements of a chunk.  At the end of chunks 0, 1, 3, 7, ... and of the row the candidates
+// are ranked against the list and each other, which is the new list, in order.  In a row of n
+// elements in no particular order about top * ln(n / chunk) elements become candidates.
+// Rows that bring more candidates than fit (ascending ones) or a NaN are taken again by slow_top,
+// whose chunks bring at most FA_TOP_MAX * 8.
+constexpr int kGroups = 256;              // first-chunk bounds (>= FA_TOP_MAX)
+constexpr int kCand = 2048;
+
+struct TopLds {
+    uint64_t list[2][FA_TOP_MAX];
+    uint64_t cand[kCand];
+    unsigned bound[kGroups];
+    unsigned count, tie;
+    uint64_t limit;
+};
+static_assert(kGroups == 256 && FA_TOP_MAX <= kGroups && kCand >= FA_TOP_MAX * 8, "sizes of the candidate lists");
+
+struct TopState {
+    int have, side;          // entries of list[side]
+    float floor;             // the list's last value once it is full
+};
+
+__device__ __forceinline__ void top_push(TopLds& l, uint64_t key) {
+    const unsigned at = atomicAdd(&l.count, 1u);
+    if (at < kCand) l.cand[at] = key;
+}
+
+// Ranks list and candidates; false if candidates were lost.  All threads, between barriers of its own.
+template <int THREADS>
+__device__ __forceinline__ bool top_refresh(TopLds& l, TopState& t, int top) {
     __syncthreads();
-    uint64_t r = lds[0];
-    for (int i = 1; i < kThreads / kWave; ++i) r = lds[i] > r ? lds[i] : r;
+    const unsigned n = l.count;
+    if (n > kCand) return false;
+    if (n) {
+        const uint64_t* cur = l.list[t.side];
+        uint64_t* next = l.list[t.side ^ 1];
+        const int total = t.have + static_cast<int>(n);
+        for (int i = threadIdx.x; i < total; i += THREADS) {
+            const uint64_t key = i < t.have ? cur[i] : l.cand[i - t.have];
+            int rank = i < t.have ? i : 0;                       // the list is in order
+            if (i >= t.have)
+                for (int j = 0; j < t.have; ++j) rank += cur[j] > key;
+            for (unsigned j = 0; j < n; ++j) rank += l.cand[j] > key;
+            if (rank < top) next[rank] = key;
+        }
+        t.side ^= 1;
+        t.have = total < top ? total : top;
+    }
     __syncthreads();
-    return r;
+    if (threadIdx.x == 0) l.count = 0;
+    if (t.have == top) t.floor = key_value(l.list[t.side][top - 1]);
+    __syncthreads();
+    return true;
+}
+
+// The top-th largest of kGroups keys' high words (group g's in l.bound[g], 0: none), the lowest
+// group first among equals; `tie` becomes the highest index the groups at that value need.
+// `first` is the caller's first index at its group's value.  The bound as a key, 0 if there are
+// fewer than `top` groups with an element.
+template <int THREADS>
+__device__ __forceinline__ uint64_t top_bound(TopLds& l, unsigned mine, int group, bool leader, int top) {
+    if (leader) l.bound[group] = mine;
+    if (threadIdx.x == 0) l.limit = 0;
+    __syncthreads();
+    if (threadIdx.x < kGroups) {
+        const unsigned v = l.bound[threadIdx.x];
+        int rank = 0;
+        for (int j = 0; j < kGroups; ++j) {
+            const unsigned o = l.bound[j];
+            rank += o > v || (o == v && j < static_cast<int>(threadIdx.x));
+        }
+        if (v && rank == top - 1) l.limit = (static_cast<uint64_t>(v) << 32) | (0xffffffffu - static_cast<unsigned>(threadIdx.x));
+    }
+    __syncthreads();
+    return l.limit;
+}
+
+// Index in the row of the first element in `mask`, one bit per element of a thread's chunk.
+template <int THREADS, int N>
+__device__ __forceinline__ int chunk_index(int place, unsigned mask) {
+    const int bit = __ffs(mask) - 1;
+    return place + (bit / N) * THREADS * N + bit % N;
+}
+
+__device__ __forceinline__ unsigned low_bits(int n) { return n >= 32 ? ~0u : (1u << n) - 1; }
+
+__device__ __forceinline__ unsigned order_of(float v) { return static_cast<unsigned>(order_key(v, 0) >> 32); }
+
+template <int DT, int THREADS>
+__device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw* x, int vocab, int top, TopLds& l, TopState& t) {
+    t = {0, 0, -kInf};
+    uint64_t low = 0;                                            // the list's last key once it is full
+    __syncthreads();
+    if (threadIdx.x == 0) l.count = 0;
+    __syncthreads();
+    constexpr int kStep = kGroups * 8;
+    for (int base = 0; base < vocab; base += kStep) {
+        uint64_t best = 0;
+        uint64_t keys[8];
+        for (int j = 0; j < 8; ++j) {
+            const int i = base + static_cast<int>(threadIdx.x) * 8 + j;
+            const bool in = threadIdx.x < kGroups && i < vocab;
+            keys[j] = in ? order_key(Elem<DT>::widen(x[i]), i) : 0;
+            if (keys[j] <= low) keys[j] = 0;
+            best = keys[j] > best ? keys[j] : best;
+        }
+        // keys are all different, so at most 8 * top elements reach the top-th of the groups' best
+        if (threadIdx.x < kGroups) l.cand[threadIdx.x] = best;
+        if (threadIdx.x == 0) l.limit = 0;
+        __syncthreads();
+        if (threadIdx.x < kGroups && best) {
+            int rank = 0;
+            for (int j = 0; j < kGroups; ++j) rank += l.cand[j] > best;
+            if (rank == top - 1) l.limit = best;
+        }
+        __syncthreads();
+        const uint64_t limit = l.limit;
+        __syncthreads();
+        for (int j = 0; j < 8; ++j)
+            if (keys[j] && keys[j] >= limit) top_push(l, keys[j]);
+        top_refresh<THREADS>(l, t, top);
+        if (t.have == top) low = l.list[t.side][top - 1];
+    }
 }
 
 struct ScoreArgs {
@@ -145,46 +393,168 @@ struct ScoreArgs {
     int64_t ignore_index;
     float *logprob, *entropy, *lse, *top_logprobs;
     int32_t* top_ids;
+    Scale scale;
 };
 
-template <int DT>
-__global__ __launch_bounds__(kThreads) void token_scores_kernel(const ScoreArgs a) {
+__device__ __forceinline__ float log_prob(const RowStat& st, const Scale& sc, float v, float lse) {
+    if (st.slow) return v == -kInf && !(st.s != st.s) ? -kInf : (v - st.m) - st.log_s;
+    const float y = fmaf(v, sc.k, -st.R) - st.log_s;             // log_s: log2 here
+    return fabsf(y) < 1e30f ? y * sc.inv_k : v - lse;
+}
+
+// One block per row: kU vectors of 16 bytes per thread and chunk, the next chunk's loads in flight
+// while one is summed.
+constexpr int kU = 4;
+
+template <int DT, int THREADS, bool TOP>
+__global__ __launch_bounds__(THREADS) void token_scores_kernel(const ScoreArgs a) {
     using E = Elem<DT>;
-    __shared__ Stat lds[kThreads / kWave];
-    __shared__ uint64_t best[kThreads / kWave];
+    using V = Vec<DT>;
+    __shared__ Acc lds[THREADS / kWave];
+    __shared__ float red[THREADS / kWave];
+    __shared__ TopLds l;
     const int64_t row = blockIdx.x;
     const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
-    const Stat st = row_stat<DT>(x, a.vocab, kLog2e, lds);
-    const float log_s = logf(st.s);
-    if (threadIdx.x == 0) {
-        a.lse[row] = st.m + log_s;
-        a.entropy[row] = st.s == 0.0f ? 0.0f : log_s - st.e * kLn2 / st.s;
-        if (a.targets) {
-            const int64_t t = a.targets[row];
-            float lp = 0.0f;
-            if (t != a.ignore_index) {
-                lp = __builtin_nanf("");
-                if (t >= 0 && t < a.vocab) {
-                    const float v = E::widen(x[t]);
-                    lp = v == -kInf && !(st.s != st.s) ? -kInf : (v - st.m) - log_s;
-                }
+    const Span sp = V::span(x, a.vocab);
+    const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
+    const int tid = threadIdx.x;
+    const float k = a.scale.k;
+    Acc acc = acc_empty();
+    TopState t = {0, 0, -kInf};
+    bool lost = false;
+    if (TOP && tid == 0) l.count = 0;
+
+    uint4 next[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+        const int i = u * THREADS + tid;
+        next[u] = i < sp.nvec ? load_once(body + i) : V::fill();
+    }
+    // one element of the row's ends per thread: head elements belong to the first chunk
+    const float head = tid < sp.head ? E::widen(x[tid]) : -kInf;
+    const float tail = tid < sp.tail ? E::widen(x[a.vocab - sp.tail + tid]) : -kInf;
+
+    int due = 1;                                                 // chunks read at the next refresh
+    int chunk = 0;
+    for (int base = 0; base < sp.nvec || chunk == 0; ++chunk) {
+        uint4 cur[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) cur[u] = next[u];
+        const int first = base;
+        base += kU * THREADS;
+        if (base < sp.nvec) {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int i = base + u * THREADS + tid;
+                next[u] = i < sp.nvec ? load_once(body + i) : V::fill();
             }
+        }
+        float v[kU * V::N];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float w[V::N];
+            V::widen(cur[u], w);
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) v[u * V::N + i] = w[i];
+        }
+        float peak = v[0];
+#pragma unroll
+        for (int i = 1; i < kU * V::N; ++i) peak = fmaxf(peak, v[i]);
+        if (chunk == 0) {
+            const float ends = fmaxf(head, tail);
+            acc_raise<true>(acc, fmaxf(acc.R, fminf(rintf(ends * k), kFar)));
+            acc_one<true>(acc, head, k);
+            acc_one<true>(acc, tail, k);
+        }
+        acc_add<true>(acc, v, peak, k);
+        if (!TOP) continue;
+        if (chunk == 0) {
+            // the bound: groups of threads (one each, or four neighbours of 1024)
+            const float top0 = fmaxf(peak, head);
+            const bool any = tid < sp.head || tid < sp.nvec;
+            unsigned mine = any ? order_of(top0) : 0;
+            constexpr int kShare = THREADS / kGroups;
+            for (int d = 1; d < kShare; d <<= 1) {
+                const unsigned o = __shfl_xor(mine, d);
+                mine = o > mine ? o : mine;
+            }
+            if (tid == 0) l.tie = 0;
+            const uint64_t limit = top_bound<THREADS>(l, mine, tid / kShare, tid % kShare == 0, a.top);
+            const float lim = limit ? key_value(limit) : -kInf;
+            const unsigned valid = low_bits(V::N * (tid < sp.nvec ? (sp.nvec - 1 - tid) / THREADS + 1 : 0));
+            const int place = sp.head + tid * V::N;
+            unsigned above = 0, equal = 0;
+#pragma unroll
+            for (int i = 0; i < kU * V::N; ++i) {
+                above |= static_cast<unsigned>(v[i] > lim) << i;
+                equal |= static_cast<unsigned>(v[i] == lim) << i;
+            }
+            above &= valid;
+            equal &= valid;
+            if (limit && static_cast<unsigned>(limit >> 32) == mine && static_cast<unsigned>(tid / kShare) <= key_index(limit)) {
+                // the groups at the bound's value: the lowest index of each has to be let in
+                int at = tid < sp.head && head == lim ? tid : equal ? chunk_index<THREADS, V::N>(place, equal) : INT32_MAX;
+                for (int d = 1; d < kShare; d <<= 1) {
+                    const int o = __shfl_xor(at, d);
+                    at = o < at ? o : at;
+                }
+                atomicMax(&l.tie, static_cast<unsigned>(at));
+            }
+            __syncthreads();
+            const int tie = limit ? static_cast<int>(l.tie) : INT32_MAX;
+            if (tid < sp.head && (head > lim || (head == lim && tid <= tie))) top_push(l, order_key(head, tid));
+            for (unsigned m = above | equal; m; m &= m - 1) {
+                const int at = chunk_index<THREADS, V::N>(place, m);
+                const float w = E::widen(x[at]);
+                if (w > lim || at <= tie) top_push(l, order_key(w, at));
+            }
+        } else if (peak > t.floor) {
+            unsigned above = 0;
+#pragma unroll
+            for (int i = 0; i < kU * V::N; ++i) above |= static_cast<unsigned>(v[i] > t.floor) << i;
+            const int place = sp.head + (first + tid) * V::N;
+            for (; above; above &= above - 1) {                  // few: read again rather than picked from registers
+                const int at = chunk_index<THREADS, V::N>(place, above);
+                top_push(l, order_key(E::widen(x[at]), at));
+            }
+        }
+        if (chunk + 1 == due && base < sp.nvec) {
+            if (!lost) lost = !top_refresh<THREADS>(l, t, a.top);
+            due *= 2;
+        }
+    }
+    if (TOP) {
+        // the last elements; before the first refresh (a row of one chunk) all of them are candidates
+        if (tid < sp.tail && (t.have < a.top || tail > t.floor))
+            top_push(l, order_key(tail, a.vocab - sp.tail + tid));
+        if (!lost) lost = !top_refresh<THREADS>(l, t, a.top);
+    }
+    acc = acc_block<true, THREADS>(acc, lds);
+    RowStat st = {acc.R, acc.s, 0.0f, log2f(acc.s), 0.0f, false};
+    st.entropy = (st.log_s - acc.e / acc.s) * a.scale.inv_k;
+    float lse = static_cast<float>((static_cast<double>(st.R) + st.log_s) * static_cast<double>(a.scale.inv_k));
+    if (!acc_good(acc)) {
+        st = slow_stat<DT, THREADS>(x, a.vocab, a.scale.inv_tau, red);
+        lse = st.m + st.log_s;
+        lost = true;
+    }
+    if (TOP && lost) slow_top<DT, THREADS>(x, a.vocab, a.top, l, t);
+    if (tid == 0) {
+        a.lse[row] = lse;
+        a.entropy[row] = st.entropy;
+        if (a.targets) {
+            const int64_t want = a.targets[row];
+            float lp = 0.0f;
+            if (want != a.ignore_index)
+                lp = want >= 0 && want < a.vocab ? log_prob(st, a.scale, E::widen(x[want]), lse) : __builtin_nanf("");
             a.logprob[row] = lp;
         }
     }
-    uint64_t prev = ~0ull;
-    for (int j = 0; j < a.top; ++j) {
-        uint64_t mine = 0;
-        for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-            const uint64_t key = order_key(E::widen(x[i]), i);
-            if (key < prev && key > mine) mine = key;
-        }
-        prev = block_max_u64(mine, best);
-        if (threadIdx.x == 0) {
-            const unsigned id = 0xffffffffu - static_cast<unsigned>(prev);
-            const float v = E::widen(x[id]);
-            a.top_ids[row * a.top + j] = static_cast<int32_t>(id);
-            a.top_logprobs[row * a.top + j] = v == -kInf && !(st.s != st.s) ? -kInf : (v - st.m) - log_s;
+    if (TOP) {
+        for (int j = tid; j < a.top; j += THREADS) {
+            const uint64_t key = l.list[t.side][j];
+            a.top_ids[row * a.top + j] = static_cast<int32_t>(key_index(key));
+            a.top_logprobs[row * a.top + j] = log_prob(st, a.scale, E::widen(x[key_index(key)]), lse);
         }
     }
 }
@@ -195,7 +565,7 @@ struct TeacherArgs {
     const float* lp;
     int64_t id_stride, lp_stride;
     int k;
-    float inv_tau, tau;
+    float tau;
     const float* row_weight;
 };
 
@@ -204,150 +574,337 @@ struct DistillArgs {
     Rows rows;
     int vocab;
     TeacherArgs t;
+    Scale scale;
     float* loss;
-    float* stat;                 // (m, log s) per row
+    float* stat;                 // FA_DISTILL_STAT floats per row: R, s, m, log s; R is NaN for a slow row
     const float* stat_in;
     const float* row_grad;
     void* grad;
     Rows grad_rows;
 };
 
-// One row's teacher, one entry per thread: t = softmax over the entries of lp / tau.
-struct Entry {
-    int id;          // -1: no entry
-    float t, log_t;
-    bool empty;      // the row has no entry with a probability
-    bool bad;        // an entry names a token outside the vocabulary
+// One row's teacher, made by the first wave alone: entries j = lane + 64 i.
+constexpr int kPer = FA_TOP_MAX / kWave;
+
+struct TeacherLds {
+    int id[FA_TOP_MAX];          // -1: nothing to write (absent, or an earlier entry has the same id)
+    float t[FA_TOP_MAX];         // probability, of all entries of the same id together
+    float x[FA_TOP_MAX];         // the student's logit
+    int empty, bad;
 };
 
-__device__ __forceinline__ float block_max_f(float v, float* lds) {
+struct Teacher {
+    float t[kPer], log_t[kPer], x[kPer];
+};
+
+__device__ __forceinline__ float wave_max_f(float v) {
+#pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float r = lds[0];
-    for (int i = 1; i < kThreads / kWave; ++i) r = fmaxf(r, lds[i]);
-    __syncthreads();
-    return r;
+    return v;
 }
 
-__device__ __forceinline__ float block_sum_f(float v, float* lds) {
+__device__ __forceinline__ float wave_sum_f(float v) {
+#pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float r = lds[0];
-    for (int i = 1; i < kThreads / kWave; ++i) r += lds[i];
-    __syncthreads();
+    return v;
+}
+
+template <int DT>
+__device__ __forceinline__ Teacher teacher_row(const TeacherArgs& a, int64_t row, const typename Elem<DT>::Raw* x, int vocab,
+                                               float inv_tau, TeacherLds& l) {
+    const int lane = threadIdx.x;
+    Teacher r;
+    int id[kPer];
+    float lp[kPer];
+    bool bad = false;
+    float peak = -kInf;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int j = lane + kWave * i;
+        id[i] = -1;
+        lp[i] = -kInf;
+        r.x[i] = -kInf;
+        if (j < a.k) {
+            id[i] = a.ids[row * a.id_stride + j];
+            if (id[i] >= 0) lp[i] = a.lp[row * a.lp_stride + j];
+            if (id[i] >= 0 && id[i] < vocab) r.x[i] = Elem<DT>::widen(x[id[i]]);
+        }
+        bad = bad || id[i] >= vocab || lp[i] != lp[i] || lp[i] == kInf;
+        peak = fmaxf(peak, lp[i]);
+    }
+    bad = __any(bad);
+    peak = wave_max_f(peak);
+    const bool empty = !bad && peak == -kInf;
+    float z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        r.log_t[i] = lp[i] == -kInf ? -kInf : (lp[i] - peak) * inv_tau;
+        r.t[i] = exp2_hw(r.log_t[i] * kLog2e);
+        z += r.t[i];
+    }
+    z = wave_sum_f(z);
+    const float log_z = logf(z), inv_z = 1.0f / z;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int j = lane + kWave * i;
+        r.log_t[i] -= log_z;
+        r.t[i] = empty ? 0.0f : r.t[i] * inv_z;
+        if (j < FA_TOP_MAX) {
+            l.id[j] = id[i] < vocab ? id[i] : -1;
+            l.t[j] = r.t[i];
+            l.x[j] = r.x[i];
+        }
+    }
+    if (lane == 0) {
+        l.empty = empty;
+        l.bad = bad;
+    }
     return r;
 }
 
-__device__ __forceinline__ Entry teacher_entry(const TeacherArgs& t, int64_t row, int vocab, float* lds) {
-    Entry e = {-1, 0.0f, 0.0f, false, false};
-    float lp = -kInf;
-    if (static_cast<int>(threadIdx.x) < t.k) {
-        e.id = t.ids[row * t.id_stride + threadIdx.x];
-        if (e.id >= 0) lp = t.lp[row * t.lp_stride + threadIdx.x];
+// Entries that name one token: the first takes their probabilities together (the gradient's term).
+__device__ __forceinline__ void teacher_unite(int k, TeacherLds& l) {
+    float sum[kPer];
+    int id[kPer];
+    __builtin_amdgcn_wave_barrier();
+    __threadfence_block();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int j = threadIdx.x + kWave * i;
+        sum[i] = 0.0f;
+        id[i] = -1;
+        if (j < k && l.id[j] >= 0) {
+            id[i] = l.id[j];
+            for (int o = 0; o < k; ++o)
+                if (l.id[o] == l.id[j]) {
+                    sum[i] += l.t[o];
+                    if (o < j) id[i] = -1;
+                }
+        }
     }
-    const bool bad = e.id >= vocab;
-    const float nan = block_sum_f(lp != lp || bad ? 1.0f : 0.0f, lds);
-    const float peak = block_max_f(lp, lds);
-    e.empty = peak == -kInf && nan == 0.0f;
-    e.bad = nan != 0.0f || peak == kInf;
-    const float d = e.empty || lp == -kInf ? -kInf : (lp - peak) * t.inv_tau;
-    const float u = exp2_hw(d * kLog2e);
-    const float z = block_sum_f(u, lds);
-    e.t = e.empty ? 0.0f : u / z;
-    e.log_t = d - logf(z);
-    return e;
+    __builtin_amdgcn_wave_barrier();
+    __threadfence_block();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int j = threadIdx.x + kWave * i;
+        if (j < k) {
+            l.id[j] = id[i];
+            l.t[j] = sum[i];
+        }
+    }
 }
 
-template <int DT>
-__device__ __forceinline__ void row_loss(const DistillArgs& a, int64_t row, const Entry& e, float xv, const Stat& st,
-                                         float weight, float* lds) {
-    const float log_s = logf(st.s);
-    float term = 0.0f;
-    if (e.t > 0.0f) {
-        const float log_q = xv == -kInf ? -kInf : (xv - st.m) * a.t.inv_tau - log_s;
-        term = e.t * (e.log_t - log_q);
+// The loss, by the first wave.
+__device__ __forceinline__ float row_loss(const DistillArgs& a, const Teacher& e, const RowStat& st, float weight, bool bad) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        if (!(e.t[i] > 0.0f)) continue;
+        float log_q;
+        if (st.slow) {
+            log_q = e.x[i] == -kInf ? -kInf : (e.x[i] - st.m) * a.scale.inv_tau - st.log_s;
+        } else {
+            const float y = fmaf(e.x[i], a.scale.k, -st.R) - st.log_s;
+            log_q = fabsf(y) < 1e30f ? y * kLn2 : e.x[i] * a.scale.inv_tau;
+        }
+        sum += e.t[i] * (e.log_t[i] - log_q);
     }
-    float loss = block_sum_f(term, lds) * (a.t.tau * a.t.tau) * weight;
-    if (e.bad || st.s != st.s) loss = __builtin_nanf("");
-    if (threadIdx.x == 0) a.loss[row] = loss;
+    sum = wave_sum_f(sum) * (a.t.tau * a.t.tau) * weight;
+    return bad || st.s != st.s ? __builtin_nanf("") : sum;
 }
 
-template <int DT>
-__device__ __forceinline__ void row_grad(const DistillArgs& a, int64_t row, const typename Elem<DT>::Raw* x,
-                                         const Entry& e, float xv, float m, float log_s, float c, float* vals,
-                                         int* ids) {
+// c * q of one element
+struct Softmax {
+    float k, R, cs;              // 2^(x k - R) * cs
+    float m, c2;                 // slow: 2^((x - m) k' - c2) * c
+    float c;
+    bool slow;
+    __device__ __forceinline__ float operator()(float v) const {
+        if (slow) return exp2_hw((v - m) * k - c2) * c;
+        return exp2_hw(fmaf(v, k, -R)) * cs;
+    }
+};
+
+__device__ __forceinline__ Softmax softmax_of(const RowStat& st, const Scale& sc, float c) {
+    Softmax f;
+    f.slow = st.slow;
+    f.k = st.slow ? sc.inv_tau * kLog2e : sc.k;
+    f.R = st.R;
+    f.cs = c / st.s;
+    f.m = st.m == -kInf ? 0.0f : st.m;
+    f.c2 = st.log_s == -kInf ? 0.0f : st.log_s * kLog2e;
+    f.c = c;
+    return f;
+}
+
+// Writes f(element) over elements [lo, hi) of a row; reads by 16 bytes, writes so where the
+// gradient's row has the same alignment.
+template <int DT, int THREADS, class F>
+__device__ __forceinline__ void map_row(const typename Elem<DT>::Raw* x, typename Elem<DT>::Raw* g, int vocab, int part,
+                                        int parts, F f) {
     using E = Elem<DT>;
-    typename E::Raw* g = static_cast<typename E::Raw*>(a.grad) + a.grad_rows.offset(row);
-    const float ref = m == -kInf ? 0.0f : m;
-    const float shift = log_s == -kInf ? 0.0f : log_s * kLog2e;
-    const float scale2 = a.t.inv_tau * kLog2e;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-        const float q = exp2_hw((E::widen(x[i]) - ref) * scale2 - shift);
-        g[i] = E::narrow(c * q);
+    using V = Vec<DT>;
+    const Span sp = V::span(x, vocab);
+    const int tid = threadIdx.x;
+    if (part == 0 && tid < sp.head) g[tid] = E::narrow(f(E::widen(x[tid])));
+    if (part == parts - 1 && tid < sp.tail) {
+        const int i = vocab - sp.tail + tid;
+        g[i] = E::narrow(f(E::widen(x[i])));
     }
-    ids[threadIdx.x] = e.id;
-    vals[threadIdx.x] = e.t;
-    __syncthreads();
-    if (e.id >= 0 && e.id < a.vocab) {
-        bool first = true;
-        float t = 0.0f;
-        for (int j = 0; j < a.t.k; ++j)
-            if (ids[j] == e.id) {
-                t += vals[j];
-                if (j < static_cast<int>(threadIdx.x)) first = false;
+    const bool same = reinterpret_cast<uintptr_t>(x) % 16 == reinterpret_cast<uintptr_t>(g) % 16;
+    const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
+    const int lo = static_cast<int>(static_cast<int64_t>(sp.nvec) * part / parts);
+    const int hi = static_cast<int>(static_cast<int64_t>(sp.nvec) * (part + 1) / parts);
+    for (int base = lo; base < hi; base += kU * THREADS) {
+        uint4 r[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int i = base + u * THREADS + tid;
+            if (i < hi) r[u] = body[i];
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int i = base + u * THREADS + tid;
+            if (i >= hi) continue;
+            float v[V::N];
+            V::widen(r[u], v);
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) v[j] = f(v[j]);
+            if (same) {
+                reinterpret_cast<uint4*>(g + sp.head)[i] = V::narrow(v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V::N; ++j) g[sp.head + i * V::N + j] = E::narrow(v[j]);
             }
-        const float q = exp2_hw((xv - ref) * scale2 - shift);
-        if (first) g[e.id] = E::narrow(c * (q - t));
+        }
     }
 }
 
+// The teacher's tokens, after the row's (or part's) other elements have been written: c (q - t).
 template <int DT>
-__device__ __forceinline__ void fill_grad(const DistillArgs& a, int64_t row, float v) {
-    typename Elem<DT>::Raw* g = static_cast<typename Elem<DT>::Raw*>(a.grad) + a.grad_rows.offset(row);
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) g[i] = Elem<DT>::narrow(v);
+__device__ __forceinline__ void fix_row(typename Elem<DT>::Raw* g, const TeacherLds& l, int k, int lo, int hi, const Softmax& f) {
+    for (int j = threadIdx.x; j < k; j += kWave) {
+        const int id = l.id[j];
+        if (id >= lo && id < hi) g[id] = Elem<DT>::narrow(f(l.x[j]) - f.c * l.t[j]);
+    }
 }
 
-template <int DT, bool LOSS, bool GRAD>
-__global__ __launch_bounds__(kThreads) void distill_kernel(const DistillArgs a) {
+template <int DT, int THREADS>
+__device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int vocab, float k) {
     using E = Elem<DT>;
-    __shared__ Stat lds[kThreads / kWave];
-    __shared__ float red[kThreads / kWave];
-    __shared__ float vals[kThreads];
-    __shared__ int ids[kThreads];
+    using V = Vec<DT>;
+    const Span sp = V::span(x, vocab);
+    const int tid = threadIdx.x;
+    const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
+    Acc acc = acc_empty();
+    if (tid < sp.head) {
+        const float v[1] = {E::widen(x[tid])};
+        acc_add<false>(acc, v, v[0], k);
+    }
+    if (tid < sp.tail) {
+        const float v[1] = {E::widen(x[vocab - sp.tail + tid])};
+        acc_add<false>(acc, v, v[0], k);
+    }
+    uint4 next[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+        const int i = u * THREADS + tid;
+        next[u] = i < sp.nvec ? body[i] : V::fill();
+    }
+    for (int base = 0; base < sp.nvec;) {
+        float v[kU * V::N];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float w[V::N];
+            V::widen(next[u], w);
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) v[u * V::N + i] = w[i];
+        }
+        base += kU * THREADS;
+        if (base < sp.nvec) {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int i = base + u * THREADS + tid;
+                next[u] = i < sp.nvec ? body[i] : V::fill();
+            }
+        }
+        float peak = v[0];
+#pragma unroll
+        for (int i = 1; i < kU * V::N; ++i) peak = fmaxf(peak, v[i]);
+        acc_add<false>(acc, v, peak, k);
+    }
+    return acc;
+}
+
+template <int DT, int THREADS, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
+    using E = Elem<DT>;
+    __shared__ Acc lds[THREADS / kWave];
+    __shared__ float red[THREADS / kWave];
+    __shared__ TeacherLds l;
     const int64_t row = blockIdx.x;
+    const int part = blockIdx.y, parts = gridDim.y;              // LOSS: one part
     const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
     const float weight = a.t.row_weight ? a.t.row_weight[row] : 1.0f;
-    const Entry e = teacher_entry(a.t, row, a.vocab, red);
     const float c = GRAD ? weight * a.t.tau * (a.row_grad ? a.row_grad[row] : 1.0f) : 0.0f;
-    if (weight == 0.0f || e.empty) {
-        if (LOSS && threadIdx.x == 0) {
-            a.loss[row] = 0.0f;
-            if (a.stat) a.stat[2 * row] = a.stat[2 * row + 1] = 0.0f;
-        }
-        if (GRAD) fill_grad<DT>(a, row, 0.0f);
-        return;
+    const bool first_wave = threadIdx.x < kWave;
+    Teacher e;
+    if (first_wave) {
+        e = teacher_row<DT>(a.t, row, x, a.vocab, a.scale.inv_tau, l);
+        if (GRAD) teacher_unite(a.t.k, l);
     }
-    const float xv = e.id >= 0 && e.id < a.vocab ? E::widen(x[e.id]) : -kInf;
-    float m, log_s;
+    RowStat st;
+    bool off = weight == 0.0f;                                   // nothing of the row's logits counts
     if (LOSS) {
-        const Stat st = row_stat<DT>(x, a.vocab, a.t.inv_tau * kLog2e, lds);
-        row_loss<DT>(a, row, e, xv, st, weight, red);
-        m = st.m;
-        log_s = logf(st.s);
-        if (a.stat && threadIdx.x == 0) {
-            a.stat[2 * row] = m;
-            a.stat[2 * row + 1] = log_s;
+        Acc acc = acc_empty();
+        if (!off) acc = sum_row<DT, THREADS>(x, a.vocab, a.scale.k);
+        acc = acc_block<false, THREADS>(acc, lds);
+        off = off || l.empty;
+        st = {acc.R, acc.s, 0.0f, log2f(acc.s), 0.0f, false};
+        if (!off && !acc_good(acc)) st = slow_stat<DT, THREADS>(x, a.vocab, a.scale.inv_tau, red);
+        if (first_wave) {
+            const float loss = off ? 0.0f : row_loss(a, e, st, weight, l.bad);
+            if (threadIdx.x == 0) {
+                a.loss[row] = loss;
+                if (a.stat) {
+                    float* o = a.stat + FA_DISTILL_STAT * row;
+                    o[0] = st.slow ? __builtin_nanf("") : st.R;
+                    o[1] = st.s;
+                    o[2] = st.m;
+                    o[3] = st.log_s;
+                }
+            }
         }
     } else {
-        m = a.stat_in[2 * row];
-        log_s = a.stat_in[2 * row + 1];
+        const float* o = a.stat_in + FA_DISTILL_STAT * row;
+        st = {o[0], o[1], o[2], o[3], 0.0f, o[0] != o[0]};
+        __syncthreads();
+        off = off || l.empty;
     }
-    if (GRAD) {
-        if (c == 0.0f || e.bad) fill_grad<DT>(a, row, e.bad ? __builtin_nanf("") : 0.0f);
-        else row_grad<DT>(a, row, x, e, xv, m, log_s, c, vals, ids);
+    if (!GRAD) return;
+    typename E::Raw* g = static_cast<typename E::Raw*>(a.grad) + a.grad_rows.offset(row);
+    if (off || c == 0.0f || l.bad) {
+        const float v = !off && l.bad ? __builtin_nanf("") : 0.0f;
+        map_row<DT, THREADS>(x, g, a.vocab, part, parts, [v](float) { return v; });
+        return;
     }
+    const Softmax f = softmax_of(st, a.scale, c);
+    map_row<DT, THREADS>(x, g, a.vocab, part, parts, f);
+    __syncthreads();
+    if (first_wave) {
+        const Span sp = Vec<DT>::span(x, a.vocab);
+        const int lo = part == 0 ? 0 : sp.head + static_cast<int>(static_cast<int64_t>(sp.nvec) * part / parts) * Vec<DT>::N;
+        const int hi = part == parts - 1 ? a.vocab : sp.head + static_cast<int>(static_cast<int64_t>(sp.nvec) * (part + 1) / parts) * Vec<DT>::N;
+        fix_row<DT>(g, l, a.t.k, lo, hi, f);
+    }
+}
+
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        const uint64_t o = __shfl_xor(static_cast<unsigned long long>(v), d);
+        v = o > v ? o : v;
+    }
+    return v;
 }
 
 // ---- merging the clients' lists -------------------------------------------------------------------
@@ -475,7 +1032,7 @@ int check_logits(const fa_logits* x) {
     if (!x || x->vocab <= 0 || x->outer < 0 || x->inner < 0) return FA_ERR_INVALID;
     if (x->dtype != FA_LOGITS_F32 && x->dtype != FA_LOGITS_BF16 && x->dtype != FA_LOGITS_F16) return FA_ERR_INVALID;
     if (x->stride_outer < 0 || x->stride_inner < 0) return FA_ERR_INVALID;
-    if (x->inner && x->outer > INT32_MAX / x->inner) return FA_ERR_TOO_LARGE;
+    if (x->vocab > FA_VOCAB_MAX || (x->inner && x->outer > INT32_MAX / x->inner)) return FA_ERR_TOO_LARGE;
     if (x->outer * x->inner && !x->data) return FA_ERR_INVALID;
     if (!aligned_to(x->data, elem_size(x->dtype))) return FA_ERR_ALIGN;
     return FA_OK;
@@ -491,30 +1048,66 @@ int check_teacher(const fa_teacher* t, int64_t rows) {
 
 Rows rows_of(const fa_logits* x) { return {x->inner, x->stride_outer, x->stride_inner}; }
 
+Scale scale_of(double temperature) {
+    Scale s;
+    s.k = static_cast<float>(1.44269504088896340736 / temperature);
+    s.inv_k = static_cast<float>(1.0 / static_cast<double>(s.k));
+    s.inv_tau = static_cast<float>(1.0 / temperature);
+    return s;
+}
+
 DistillArgs distill_args(const fa_logits* x, const fa_teacher* t) {
     DistillArgs a = {};
     a.x = x->data;
     a.rows = rows_of(x);
     a.vocab = x->vocab;
-    a.t = {t->ids, t->logprobs, t->id_stride, t->lp_stride, t->k, static_cast<float>(1.0 / t->temperature),
-           static_cast<float>(t->temperature), t->row_weight};
+    a.t = {t->ids, t->logprobs, t->id_stride, t->lp_stride, t->k, static_cast<float>(t->temperature), t->row_weight};
+    a.scale = scale_of(t->temperature);
     return a;
+}
+
+// Few long rows: one block of 1024 threads each; else 256.
+bool wide_blocks(int64_t rows, int vocab) { return rows < 512 && vocab >= 8192; }
+
+template <int DT, bool LOSS, bool GRAD>
+void launch_distill_t(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
+    const int64_t rows = x->outer * x->inner;
+    int parts = 1;
+    if (!LOSS) {                 // a gradient alone has nothing to sum: a row may be cut
+        while (parts < 64 && rows * parts < 2048 && x->vocab / parts >= 8192) parts *= 2;
+    }
+    const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(parts));
+    if (LOSS && wide_blocks(rows, x->vocab))
+        hipLaunchKernelGGL((distill_kernel<DT, 1024, LOSS, GRAD>), grid, dim3(1024), 0, st, a);
+    else
+        hipLaunchKernelGGL((distill_kernel<DT, 256, LOSS, GRAD>), grid, dim3(256), 0, st, a);
 }
 
 template <bool LOSS, bool GRAD>
 int launch_distill(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
-    const unsigned rows = static_cast<unsigned>(x->outer * x->inner);
     switch (x->dtype) {
-        case FA_LOGITS_F32:
-            hipLaunchKernelGGL((distill_kernel<FA_LOGITS_F32, LOSS, GRAD>), dim3(rows), dim3(kThreads), 0, st, a);
-            break;
-        case FA_LOGITS_BF16:
-            hipLaunchKernelGGL((distill_kernel<FA_LOGITS_BF16, LOSS, GRAD>), dim3(rows), dim3(kThreads), 0, st, a);
-            break;
-        default:
-            hipLaunchKernelGGL((distill_kernel<FA_LOGITS_F16, LOSS, GRAD>), dim3(rows), dim3(kThreads), 0, st, a);
+        case FA_LOGITS_F32: launch_distill_t<FA_LOGITS_F32, LOSS, GRAD>(x, a, st); break;
+        case FA_LOGITS_BF16: launch_distill_t<FA_LOGITS_BF16, LOSS, GRAD>(x, a, st); break;
+        default: launch_distill_t<FA_LOGITS_F16, LOSS, GRAD>(x, a, st);
     }
     return hip_code(hipGetLastError());
+}
+
+template <int DT, int THREADS>
+void launch_scores_t(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(x->outer * x->inner));
+    if (a.top)
+        hipLaunchKernelGGL((token_scores_kernel<DT, THREADS, true>), grid, dim3(THREADS), 0, st, a);
+    else
+        hipLaunchKernelGGL((token_scores_kernel<DT, THREADS, false>), grid, dim3(THREADS), 0, st, a);
+}
+
+template <int DT>
+void launch_scores(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
+    if (wide_blocks(x->outer * x->inner, x->vocab))
+        launch_scores_t<DT, 1024>(x, a, st);
+    else
+        launch_scores_t<DT, 256>(x, a, st);
 }
 
 hipStream_t as_stream(fa_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
@@ -541,17 +1134,11 @@ int fa_token_scores(const fa_logits* x, const int64_t* targets, int64_t ignore_i
     if (!entropy || !lse || (targets && !logprob) || (top && (!top_ids || !top_logprobs))) return FA_ERR_INVALID;
     (void)ws;
     const ScoreArgs a = {x->data, rows_of(x), x->vocab, top, targets, ignore_index, logprob, entropy, lse,
-                         top_logprobs, top_ids};
-    const dim3 grid(static_cast<unsigned>(rows));
+                         top_logprobs, top_ids, scale_of(1.0)};
     switch (x->dtype) {
-        case FA_LOGITS_F32:
-            hipLaunchKernelGGL(token_scores_kernel<FA_LOGITS_F32>, grid, dim3(kThreads), 0, as_stream(stream), a);
-            break;
-        case FA_LOGITS_BF16:
-            hipLaunchKernelGGL(token_scores_kernel<FA_LOGITS_BF16>, grid, dim3(kThreads), 0, as_stream(stream), a);
-            break;
-        default:
-            hipLaunchKernelGGL(token_scores_kernel<FA_LOGITS_F16>, grid, dim3(kThreads), 0, as_stream(stream), a);
+        case FA_LOGITS_F32: launch_scores<FA_LOGITS_F32>(x, a, as_stream(stream)); break;
+        case FA_LOGITS_BF16: launch_scores<FA_LOGITS_BF16>(x, a, as_stream(stream)); break;
+        default: launch_scores<FA_LOGITS_F16>(x, a, as_stream(stream));
     }
     return hip_code(hipGetLastError());
 }

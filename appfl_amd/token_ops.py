@@ -71,7 +71,7 @@ def _logits(x: torch.Tensor) -> N.Logits:
     else:
         raise ValueError(f"logits must be [rows, vocab] or [batch, rows, vocab], got shape {tuple(x.shape)}")
     vocab = x.shape[-1]
-    if vocab < 1 or vocab > 0x7FFFFFFF:
+    if vocab < 1 or vocab > N.FA_VOCAB_MAX:
         raise ValueError(f"a vocabulary of {vocab} tokens")
     if x.stride(-1) != 1 and vocab > 1:
         raise ValueError("logits must have adjacent elements along the vocabulary")
@@ -211,7 +211,7 @@ class _Distill(torch.autograd.Function):
         device = logits.device
         with _on(device):
             loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-            stat = torch.empty(logits.shape[:-1] + (2,), dtype=torch.float32, device=device)
+            stat = torch.empty(logits.shape[:-1] + (N.FA_DISTILL_STAT,), dtype=torch.float32, device=device)
             ws = _workspace(x, 0, device)
             N.check(N.load().fa_distill_loss(C.byref(x), C.byref(t), loss.data_ptr(), stat.data_ptr(), _ptr(ws),
                                              _stream(logits)), "fa_distill_loss")

@@ -497,6 +497,8 @@ int fa_synth_fill(float* p, const float* base, size_t n, uint64_t seed, uint64_t
  *   - per-row results are written in row order, packed.
  */
 enum { FA_LOGITS_F32 = 0, FA_LOGITS_BF16 = 1, FA_LOGITS_F16 = 2 };
+#define FA_VOCAB_MAX (1 << 30) /* tokens of a vocabulary                                      */
+#define FA_DISTILL_STAT 4      /* floats per row that fa_distill_loss leaves for the gradient */
 #define FA_TOP_MAX 256         /* entries of one list                                         */
 #define FA_MERGE_CLIENTS 128   /* clients of one fa_merge_tops call                           */
 #define FA_MERGE_ENTRIES 8192  /* clients * entries of one list of one fa_merge_tops call     */
@@ -560,7 +562,7 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
  * q = softmax over the vocabulary of x / T, per row
  *   loss = weight * T^2 * sum_j t_j (log t_j - log q[id_j])
  *   d loss / d x_v = weight * T * (q_v - sum_{j: id_j = v} t_j)
- * fa_distill_loss writes the losses and, for the backward call, `stat` (2 floats per row);
+ * fa_distill_loss writes the losses and, for the backward call, `stat` (FA_DISTILL_STAT floats a row);
  * fa_distill_grad writes the gradient of sum_r row_grad[r] * loss[r] (row_grad NULL: 1);
  * fa_distill_loss_grad does both (row_grad 1) and may write the gradient over the logits (same
  * data and strides).  The gradient has the logits' type and row shape, with strides of its own;
