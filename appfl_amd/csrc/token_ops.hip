@@ -14,7 +14,6 @@
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kWave = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -899,125 +898,243 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     }
 }
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-    for (int d = kWave / 2; d > 0; d >>= 1) {
-        const uint64_t o = __shfl_xor(static_cast<unsigned long long>(v), d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-
 // ---- merging the clients' lists -------------------------------------------------------------------
+// One block per row, every entry in a register of its thread.  Entries are grouped by a hash table in
+// LDS.  A group's probabilities are added as whole numbers, scaled by the power of two that puts the
+// group's largest below 2^51: at most 2^13 entries stay below 2^64, whole numbers add up to the same
+// sum in any order, and a sum is off by no more than 2^-51 of the largest term per entry (fp64
+// additions: 2^-53 of the sum each).  The groups' values are then ranked, ties to the lowest id.
+// A table takes kFull<THREADS> different tokens; a row with more is merged in rounds, each of which
+// takes the tokens that got into the table and ranks them together with the best of the rounds
+// before.
 struct MergeArgs {
     const int32_t* ids;
     const float* lp;
     int64_t id_client, id_row, lp_client, lp_row;
     const float* unit;
     int64_t unit_client, unit_row;
-    int K, k, top, n2;           // n2: K * k rounded up to a power of two
+    int K, k, top;
+    uint64_t per_k;              // 2^32 / k, rounded up: i / k for i * k < 2^32
     int32_t* out_ids;
     float* out_lp;
     double w[FA_MERGE_CLIENTS];
 };
 
-__global__ __launch_bounds__(kThreads) void merge_tops_kernel(const MergeArgs a) {
-    extern __shared__ uint64_t dyn[];
-    __shared__ int answered[FA_MERGE_CLIENTS];
-    __shared__ uint64_t red[kThreads / kWave];
-    uint64_t* key = dyn;                                   // (id, position), position in client order
-    double* p = reinterpret_cast<double*>(dyn + a.n2);     // by position
+struct Ranked {
+    uint64_t key;                // the value's bits; a NaN's are the largest
+    unsigned id;
+};
+
+__device__ __forceinline__ bool before(uint64_t ka, unsigned ia, uint64_t kb, unsigned ib) {
+    return ka > kb || (ka == kb && ia < ib);
+}
+
+template <int THREADS>
+struct MergeLds {
+    static constexpr int kSlots = 4 * THREADS;
+    static constexpr int kFull = 3 * THREADS;      // tokens after which none is added; THREADS more may be under way
+    double share[FA_MERGE_CLIENTS];
+    unsigned answered[FA_MERGE_CLIENTS / 32];
+    unsigned token[kSlots];                        // id, ~0: free
+    unsigned peak[kSlots];                         // exponent of the group's largest term
+    uint64_t sum[kSlots];
+    uint64_t key[kSlots + FA_TOP_MAX];             // by group, in the order of their coming, then the list so far
+    unsigned id[kSlots + FA_TOP_MAX];
+    u16 slot[kSlots];                              // by group
+    uint64_t bound[THREADS];
+    unsigned bound_id[THREADS];
+    unsigned count, open, kept;
+    uint64_t limit;
+    unsigned limit_id;
+    double total;
+};
+
+constexpr unsigned kFree = ~0u;
+constexpr unsigned kExpInf = 2047;
+
+template <int THREADS>
+__device__ __forceinline__ int find_slot(const MergeLds<THREADS>& l, unsigned id, unsigned& at) {
+    // the slot of `id` (>= 0), or -1 with `at` the free slot met first, or at = kFree in a full table
+    constexpr unsigned kMask = MergeLds<THREADS>::kSlots - 1;
+    for (unsigned n = 0; n <= kMask; ++n) {
+        const unsigned t = __hip_atomic_load(&l.token[at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (t == id) return static_cast<int>(at);
+        if (t == kFree) return -1;
+        at = (at + 1) & kMask;
+    }
+    at = kFree;
+    return -1;
+}
+
+template <int THREADS>
+__device__ __forceinline__ unsigned hash_of(unsigned id) {
+    constexpr int kBits = __builtin_ctz(MergeLds<THREADS>::kSlots);
+    return (id * 0x9e3779b1u) >> (32 - kBits);
+}
+
+// PER entries per thread
+template <int THREADS, int PER>
+__global__ __launch_bounds__(THREADS, PER <= 16 ? 4 : 2) void merge_tops_kernel(const MergeArgs a) {
+    using L = MergeLds<THREADS>;
+    __shared__ L l;
     const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x;
     const int n = a.K * a.k;
-    for (int c = threadIdx.x; c < FA_MERGE_CLIENTS; c += kThreads) answered[c] = 0;
+    for (int c = tid; c < a.K; c += THREADS)
+        l.share[c] = a.w[c] * static_cast<double>(a.unit ? a.unit[c * a.unit_client + row * a.unit_row] : 1.0f);
+    if (tid < FA_MERGE_CLIENTS / 32) l.answered[tid] = 0;
+    for (int i = tid; i < L::kSlots; i += THREADS) {
+        l.token[i] = kFree;
+        l.peak[i] = 0;
+        l.sum[i] = 0;
+    }
+    if (tid == 0) l.count = l.open = l.kept = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < a.n2; i += kThreads) {
-        uint64_t kk = ~0ull;
-        double v = -1.0;
+
+    unsigned id[PER];
+    double p[PER];
+    int slot[PER];                                 // -1: waiting, -2: absent or done
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int i = tid + e * THREADS;
+        slot[e] = -2;
+        id[e] = 0;
+        p[e] = 0.0;
         if (i < n) {
-            const int c = i / a.k, j = i - c * a.k;
-            const float u = a.unit ? a.unit[c * a.unit_client + row * a.unit_row] : 1.0f;
-            const double share = a.w[c] * static_cast<double>(u);
-            const int id = a.ids[c * a.id_client + row * a.id_row + j];
-            if (id >= 0 && share > 0.0) {
-                v = share * exp(static_cast<double>(a.lp[c * a.lp_client + row * a.lp_row + j]));
-                if (v != v) v = __builtin_nan("");
-                kk = (static_cast<uint64_t>(static_cast<unsigned>(id)) << 32) | static_cast<unsigned>(i);
-                answered[c] = 1;
+            const int c = static_cast<int>((static_cast<uint64_t>(i) * a.per_k) >> 32), j = i - c * a.k;
+            const int v = a.ids[c * a.id_client + row * a.id_row + j];
+            const float lp = a.lp[c * a.lp_client + row * a.lp_row + j];
+            const double share = l.share[c];
+            if (v >= 0 && share > 0.0) {
+                id[e] = static_cast<unsigned>(v);
+                p[e] = share * exp(static_cast<double>(lp));
+                slot[e] = -1;
+                atomicOr(&l.answered[c / 32], 1u << (c % 32));
             }
         }
-        key[i] = kk;
-        p[i] = v;
     }
-    for (int size = 2; size <= a.n2; size <<= 1)
-        for (int d = size >> 1; d > 0; d >>= 1) {
+    int have = 0;
+    for (bool more = true; more;) {
+        // tokens into the table
+        bool waiting = false;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            if (slot[e] != -1) continue;
+            unsigned at = hash_of<THREADS>(id[e]);
+            for (;;) {
+                const int s = find_slot(l, id[e], at);
+                if (s >= 0) {
+                    slot[e] = s;
+                    break;
+                }
+                if (at == kFree || __hip_atomic_load(&l.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) >= L::kFull) break;
+                const unsigned old = atomicCAS(&l.token[at], kFree, id[e]);
+                if (old == kFree) {
+                    l.slot[atomicAdd(&l.count, 1u)] = static_cast<u16>(at);
+                    slot[e] = static_cast<int>(at);
+                    break;
+                }                                  // taken meanwhile, perhaps by this very token: look again
+            }
+            if (slot[e] >= 0)
+                atomicMax(&l.peak[slot[e]], static_cast<unsigned>(__double2hiint(p[e])) >> 20 & 2047u);
+            else
+                waiting = true;
+        }
+        if (waiting) l.open = 1;
+        __syncthreads();
+        more = l.open != 0;
+        const int groups = static_cast<int>(l.count);
+        if (more) {
+            // entries that found no room: their token may have come in through another entry
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                if (slot[e] != -1) continue;
+                unsigned at = hash_of<THREADS>(id[e]);
+                const int s = find_slot(l, id[e], at);
+                if (s < 0) continue;
+                slot[e] = s;
+                atomicMax(&l.peak[s], static_cast<unsigned>(__double2hiint(p[e])) >> 20 & 2047u);
+            }
             __syncthreads();
-            for (int i = threadIdx.x; i < a.n2 / 2; i += kThreads) {
-                const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
-                const bool up = (lo & size) == 0;
-                const uint64_t x = key[lo], y = key[hi];
-                if ((x > y) == up) {
-                    key[lo] = y;
-                    key[hi] = x;
+        }
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            if (slot[e] < 0) continue;
+            const unsigned x = l.peak[slot[e]];
+            unsigned long long q;
+            if (x == kExpInf) {                    // counts of NaN and of infinities
+                q = p[e] != p[e] ? 1ull << 32 : p[e] > 1.7976931348623157e308 ? 1ull : 0ull;
+            } else {
+                // 2^51 above the peak's binade; adding 2^52 leaves the whole number in the low bits
+                const double scaled = ldexp(p[e], 51 + 1022 - static_cast<int>(x ? x : 1));
+                q = static_cast<unsigned long long>(__double_as_longlong(scaled + 4503599627370496.0)) & 0xfffffffffffffull;
+            }
+            atomicAdd(reinterpret_cast<unsigned long long*>(&l.sum[slot[e]]), q);
+            slot[e] = -2;
+        }
+        __syncthreads();
+        // the groups' values, behind them the list so far
+        for (int g = tid; g < groups; g += THREADS) {
+            const int s = l.slot[g];
+            const unsigned x = l.peak[s];
+            const uint64_t sum = l.sum[s];
+            double v;
+            if (x == kExpInf)
+                v = sum >> 32 ? __builtin_nan("") : __builtin_inf();
+            else
+                v = ldexp(static_cast<double>(sum), static_cast<int>(x ? x : 1) - 1022 - 51);
+            l.key[g] = v != v ? 0x7ff8000000000000ull : static_cast<uint64_t>(__double_as_longlong(v));
+            l.id[g] = l.token[s];
+            l.token[s] = kFree;
+            l.peak[s] = 0;
+            l.sum[s] = 0;
+        }
+        const int kept = static_cast<int>(l.kept);
+        for (int j = tid; j < kept; j += THREADS) {
+            l.key[groups + j] = l.bound[j];
+            l.id[groups + j] = l.bound_id[j];
+        }
+        __syncthreads();
+        const int total = groups + kept;
+        have = total < a.top ? total : a.top;
+        // ranks
+        for (int g = tid; g < total; g += THREADS) {
+            const uint64_t key = l.key[g];
+            const unsigned me = l.id[g];
+            int rank = 0;
+            for (int o = 0; o < total; ++o) rank += before(l.key[o], l.id[o], key, me);
+            if (rank < a.top) {
+                if (more) {
+                    l.bound[rank] = key;
+                    l.bound_id[rank] = me;
+                } else {
+                    a.out_ids[row * a.top + rank] = static_cast<int32_t>(me);
+                    l.bound[rank] = key;
                 }
             }
         }
-    __syncthreads();
-    double total = 0.0;
-    for (int c = 0; c < a.K; ++c)
-        if (answered[c]) total += a.w[c] * static_cast<double>(a.unit ? a.unit[c * a.unit_client + row * a.unit_row] : 1.0f);
-    for (int i = threadIdx.x; i < a.n2; i += kThreads) {
-        if (key[i] == ~0ull) continue;
-        const unsigned id = static_cast<unsigned>(key[i] >> 32);
-        if (i && static_cast<unsigned>(key[i - 1] >> 32) == id) continue;
-        double s = 0.0;                                    // a run's slots belong to its first entry
-        for (int j = i; j < a.n2 && static_cast<unsigned>(key[j] >> 32) == id; ++j) {
-            const unsigned pos = static_cast<unsigned>(key[j]);
-            s += p[pos];
-            p[pos] = -1.0;
+        if (tid == 0) {
+            l.count = l.open = 0;
+            l.kept = have;
         }
-        p[static_cast<unsigned>(key[i])] = s;
+        __syncthreads();
+    }
+    if (tid < kWave) {
+        double t = 0.0;
+        for (int c = tid; c < a.K; c += kWave)
+            if (l.answered[c / 32] >> (c % 32) & 1) t += l.share[c];
+        for (int d = kWave / 2; d > 0; d >>= 1) t += __shfl_xor(t, d);
+        if (tid == 0) l.total = t;
     }
     __syncthreads();
-    for (int t = 0; t < a.top; ++t) {
-        // largest value, then (among equals) the first place in the order of ids
-        int64_t best = -1;
-        int at = 0;
-        for (int i = threadIdx.x; i < a.n2; i += kThreads) {
-            if (key[i] == ~0ull) continue;
-            const double v = p[static_cast<unsigned>(key[i])];
-            const int64_t b = v != v ? 0x7ff8000000000000ll : __double_as_longlong(v);
-            if (b > best) {
-                best = b;
-                at = i;
-            }
-        }
-        const uint64_t v1 = best < 0 ? 0 : static_cast<uint64_t>(best) + 1;
-        uint64_t top = wave_max_u64(v1);
-        if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = top;
-        __syncthreads();
-        top = red[0];
-        for (int i = 1; i < kThreads / kWave; ++i) top = red[i] > top ? red[i] : top;
-        __syncthreads();
-        uint64_t place = v1 == top && top ? ~static_cast<uint64_t>(at) : 0;
-        place = wave_max_u64(place);
-        if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = place;
-        __syncthreads();
-        place = red[0];
-        for (int i = 1; i < kThreads / kWave; ++i) place = red[i] > place ? red[i] : place;
-        if (threadIdx.x == 0) {
-            int32_t id = -1;
-            float lp = -kInf;
-            if (top) {
-                const unsigned i = static_cast<unsigned>(~place);
-                const unsigned pos = static_cast<unsigned>(key[i]);
-                id = static_cast<int32_t>(key[i] >> 32);
-                lp = static_cast<float>(log(p[pos] / total));
-                p[pos] = -1.0;
-            }
-            a.out_ids[row * a.top + t] = id;
-            a.out_lp[row * a.top + t] = lp;
-        }
-        __syncthreads();
+    const double total = l.total;
+    for (int j = tid; j < a.top; j += THREADS) {
+        float lp = -kInf;
+        if (j < have)
+            lp = static_cast<float>(log(__longlong_as_double(static_cast<long long>(l.bound[j])) / total));
+        else
+            a.out_ids[row * a.top + j] = -1;
+        a.out_lp[row * a.top + j] = lp;
     }
 }
 
@@ -1112,6 +1229,22 @@ void launch_scores(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
 
 hipStream_t as_stream(fa_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
+template <int THREADS, int PER>
+void launch_merge_t(const MergeArgs& a, int64_t rows, hipStream_t st) {
+    hipLaunchKernelGGL((merge_tops_kernel<THREADS, PER>), dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, st, a);
+}
+
+int launch_merge(const MergeArgs& a, int64_t rows, hipStream_t st) {
+    const int n = a.K * a.k;
+    if (n <= 256) launch_merge_t<256, 1>(a, rows, st);
+    else if (n <= 512) launch_merge_t<256, 2>(a, rows, st);
+    else if (n <= 1024) launch_merge_t<256, 4>(a, rows, st);
+    else if (n <= 2048) launch_merge_t<256, 8>(a, rows, st);
+    else if (n <= 4096) launch_merge_t<256, 16>(a, rows, st);
+    else launch_merge_t<256, 32>(a, rows, st);
+    return hip_code(hipGetLastError());
+}
+
 }  // namespace
 
 extern "C" {
@@ -1192,7 +1325,7 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
                   float* out_logprobs, fa_stream_t stream) {
     if (!in || !w || K < 1 || K > FA_MERGE_CLIENTS || rows < 0 || in->k < 1 || in->k > FA_TOP_MAX) return FA_ERR_INVALID;
     if (static_cast<int64_t>(K) * in->k > FA_MERGE_ENTRIES || rows > INT32_MAX) return FA_ERR_TOO_LARGE;
-    if (top < 1 || top > K * in->k) return FA_ERR_INVALID;
+    if (top < 1 || top > K * in->k || top > FA_TOP_MAX) return FA_ERR_INVALID;
     if (in->id_client < 0 || in->id_row < 0 || in->lp_client < 0 || in->lp_row < 0 || in->unit_client < 0 ||
         in->unit_row < 0)
         return FA_ERR_INVALID;
@@ -1213,17 +1346,11 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
     a.K = K;
     a.k = in->k;
     a.top = top;
-    a.n2 = 1;
-    while (a.n2 < K * in->k) a.n2 *= 2;
+    a.per_k = ((1ull << 32) + in->k - 1) / in->k;
     a.out_ids = out_ids;
     a.out_lp = out_logprobs;
     for (int c = 0; c < K; ++c) a.w[c] = w[c];
-    const unsigned lds = static_cast<unsigned>(a.n2) * 16;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(merge_tops_kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, FA_MERGE_ENTRIES * 16);
-    if (e != hipSuccess) return hip_code(e);
-    hipLaunchKernelGGL(merge_tops_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), lds, as_stream(stream), a);
-    return hip_code(hipGetLastError());
+    return launch_merge(a, rows, as_stream(stream));
 }
 
 }  // extern "C"

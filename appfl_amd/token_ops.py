@@ -160,8 +160,8 @@ def merge_tops(ids: torch.Tensor, logprobs: torch.Tensor, weights: Sequence[floa
         raise ValueError("client weights must be finite and not negative")
     if not isinstance(top, int) or isinstance(top, bool):
         raise TypeError("top must be an int")
-    if not 1 <= top <= K * k:
-        raise ValueError(f"top must be in 1..{K * k}, got {top}")
+    if not 1 <= top <= min(K * k, TOP_MAX):
+        raise ValueError(f"top must be in 1..{min(K * k, TOP_MAX)}, got {top}")
     unit_client = unit_row = 0
     if token_weight is not None:
         _on_device("token_weight", token_weight, device)

@@ -548,11 +548,12 @@ int fa_token_scores(const fa_logits* logits, const int64_t* targets, int64_t ign
 /*
  * Weighted mean of K clients' answers, cut to its `top` largest entries:
  *   p(v) = sum_c w_c u_c exp(lp_c(v)) / sum_{c answering} w_c u_c
- * in fp64, clients in order c = 0..K-1, entries of one client in list order (an id listed twice
- * counts twice).  w: HOST array of K finite weights >= 0; u: token_weight.  A client whose w_c u_c
- * is not above zero, or whose list is empty, does not answer that row.  Output best first, equal
- * values by the lower id first; id -1 and -inf where a row has fewer than `top` different tokens.
- * 1 <= top <= K * k.
+ * w: HOST array of K finite weights >= 0; u: token_weight.  Terms are fp64 and added without regard
+ * to their order (a token's sum is off by at most 2^-51 of its largest term per entry); an id that a
+ * client lists twice counts twice.  A client whose w_c u_c is not above zero, or whose list is
+ * empty, does not answer that row.  Output best first, equal values by the lower id first; id -1 and
+ * -inf where a row has fewer than `top` different tokens.
+ * 1 <= top <= min(K * k, FA_TOP_MAX).
  */
 int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int top, int32_t* out_ids,
                   float* out_logprobs, fa_stream_t stream);
