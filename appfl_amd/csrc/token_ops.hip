@@ -88,6 +88,11 @@ struct Vec {
             }
         }
     }
+    // The same for a value that was widened before: costs less than the registers to keep it.
+    static __device__ __forceinline__ void widen_again(uint4 r, float (&v)[N]) {
+        asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
+        widen(r, v);
+    }
     static __device__ __forceinline__ uint4 narrow(const float (&v)[N]) {
         unsigned w[4];
 #pragma unroll
@@ -100,6 +105,14 @@ struct Vec {
         return {w[0], w[1], w[2], w[3]};
     }
 };
+
+template <int N>
+__device__ __forceinline__ float max_of(const float (&v)[N]) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+    return m;
+}
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -114,6 +127,8 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 // multiply-add rounds once, relative to its small result, rescaling by a power of two is exact, and
 // the rounding of k is a change of T by 2^-25 that all of a row's terms share.
 //   s = sum 2^(x k - R),   e = sum 2^(x k - R) (x k - R)   (entropy = (log2 s - e / s) / k)
+// R is raised only when a value passes it by more than 2^kSlack: terms are then at most that large,
+// which fp32 does not mind.
 // R stays within +-kFar, so a distance is finite; a row whose x k lies beyond (a row of the type's
 // lowest value, infinities) or holds a NaN ends with s = 0, inf or NaN and is taken again by
 // slow_stat, which subtracts the maximum before it scales.
@@ -144,10 +159,13 @@ __device__ __forceinline__ void acc_one(Acc& a, float v, float k) {
     if (ENT) a.e = fmaf(t, fmaxf(y, -200.0f), a.e);       // 0 * -inf; a NaN stays in t
 }
 
+constexpr float kSlack = 8.0f;
+
 // N terms whose largest is `top`
 template <bool ENT, int N>
 __device__ __forceinline__ void acc_add(Acc& a, const float (&v)[N], float top, float k) {
-    acc_raise<ENT>(a, fmaxf(a.R, fminf(rintf(top * k), kFar)));
+    const float y = top * k;
+    if (__any(y > a.R + kSlack)) acc_raise<ENT>(a, fmaxf(a.R, fminf(rintf(y), kFar)));
 #pragma unroll
     for (int i = 0; i < N; ++i) acc_one<ENT>(a, v[i], k);
 }
@@ -255,133 +273,261 @@ __device__ __forceinline__ float key_value(uint64_t key) {       // not for a Na
 }
 
 // ---- the top entries of a row ---------------------------------------------------------------------
-// One pass.  The row is read in chunks of adjacent elements.  From the first chunk every thread
-// contributes its largest key; the top-th largest of those is a bound that at least `top` elements
-// reach, and the elements that reach it become candidates.  From then on only elements above the
-// current top-th value are candidates (an equal one has a higher index), found by comparing the
-// largest of a thread's elements of a chunk.  At the end of chunks 0, 1, 3, 7, ... and of the row the candidates
-// are ranked against the list and each other, which is the new list, in order.  In a row of n
-// elements in no particular order about top * ln(n / chunk) elements become candidates.
-// Rows that bring more candidates than fit (ascending ones) or a NaN are taken again by slow_top,
-// whose chunks bring at most FA_TOP_MAX * 8.
-constexpr int kGroups = 256;              // first-chunk bounds (>= FA_TOP_MAX)
-constexpr int kCand = 2048;
-
+// One pass.  The row is read in chunks of adjacent elements.  From the first chunk every group of
+// threads contributes its largest value; the top-th largest of those is a bound that at least `top`
+// elements reach, and the elements that reach it become candidates, in a buffer of their wave.  From
+// then on only elements above the floor -- a value that `top` elements before them reach -- are
+// candidates (an equal one has a higher index), found by comparing the largest of a vector's elements.
+// The floor is raised after chunks 1, 3, 7, ... and at the end: with W waves, the least of the waves'
+// ceil(top / W)-th largest candidates.  Candidates below it are dropped; in a row in no particular
+// order about top * (1 + ln(n / chunk)) elements ever become candidates.  The last ones are ranked
+// against each other.
+// A row that brings more candidates than fit (an ascending one) or holds a NaN is taken again by
+// slow_top, whose steps bring at most 8 * top.
+template <int THREADS>
 struct TopLds {
-    uint64_t list[2][FA_TOP_MAX];
-    uint64_t cand[kCand];
+    static constexpr int kWaves = THREADS / kWave;
+    static constexpr int kGroups = THREADS < 256 ? THREADS : 256;       // >= the largest `top`
+    static constexpr int kRoom = kWaves == 16 ? 192 : 512;
+    uint64_t cand[kWaves * kRoom];
+    uint64_t list[kGroups];
     unsigned bound[kGroups];
-    unsigned count, tie;
-    uint64_t limit;
+    int held[kWaves];
+    float floor[kWaves];
+    unsigned limit, limit_group, tie, count;
+    uint64_t reach;
+    static_assert(kWaves * kRoom >= kGroups * 8, "a step of slow_top");
 };
-static_assert(kGroups == 256 && FA_TOP_MAX <= kGroups && kCand >= FA_TOP_MAX * 8, "sizes of the candidate lists");
-
-struct TopState {
-    int have, side;          // entries of list[side]
-    float floor;             // the list's last value once it is full
-};
-
-__device__ __forceinline__ void top_push(TopLds& l, uint64_t key) {
-    const unsigned at = atomicAdd(&l.count, 1u);
-    if (at < kCand) l.cand[at] = key;
-}
-
-// Ranks list and candidates; false if candidates were lost.  All threads, between barriers of its own.
-template <int THREADS>
-__device__ __forceinline__ bool top_refresh(TopLds& l, TopState& t, int top) {
-    __syncthreads();
-    const unsigned n = l.count;
-    if (n > kCand) return false;
-    if (n) {
-        const uint64_t* cur = l.list[t.side];
-        uint64_t* next = l.list[t.side ^ 1];
-        const int total = t.have + static_cast<int>(n);
-        for (int i = threadIdx.x; i < total; i += THREADS) {
-            const uint64_t key = i < t.have ? cur[i] : l.cand[i - t.have];
-            int rank = i < t.have ? i : 0;                       // the list is in order
-            if (i >= t.have)
-                for (int j = 0; j < t.have; ++j) rank += cur[j] > key;
-            for (unsigned j = 0; j < n; ++j) rank += l.cand[j] > key;
-            if (rank < top) next[rank] = key;
-        }
-        t.side ^= 1;
-        t.have = total < top ? total : top;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) l.count = 0;
-    if (t.have == top) t.floor = key_value(l.list[t.side][top - 1]);
-    __syncthreads();
-    return true;
-}
-
-// The top-th largest of kGroups keys' high words (group g's in l.bound[g], 0: none), the lowest
-// group first among equals; `tie` becomes the highest index the groups at that value need.
-// `first` is the caller's first index at its group's value.  The bound as a key, 0 if there are
-// fewer than `top` groups with an element.
-template <int THREADS>
-__device__ __forceinline__ uint64_t top_bound(TopLds& l, unsigned mine, int group, bool leader, int top) {
-    if (leader) l.bound[group] = mine;
-    if (threadIdx.x == 0) l.limit = 0;
-    __syncthreads();
-    if (threadIdx.x < kGroups) {
-        const unsigned v = l.bound[threadIdx.x];
-        int rank = 0;
-        for (int j = 0; j < kGroups; ++j) {
-            const unsigned o = l.bound[j];
-            rank += o > v || (o == v && j < static_cast<int>(threadIdx.x));
-        }
-        if (v && rank == top - 1) l.limit = (static_cast<uint64_t>(v) << 32) | (0xffffffffu - static_cast<unsigned>(threadIdx.x));
-    }
-    __syncthreads();
-    return l.limit;
-}
-
-// Index in the row of the first element in `mask`, one bit per element of a thread's chunk.
-template <int THREADS, int N>
-__device__ __forceinline__ int chunk_index(int place, unsigned mask) {
-    const int bit = __ffs(mask) - 1;
-    return place + (bit / N) * THREADS * N + bit % N;
-}
-
-__device__ __forceinline__ unsigned low_bits(int n) { return n >= 32 ? ~0u : (1u << n) - 1; }
 
 __device__ __forceinline__ unsigned order_of(float v) { return static_cast<unsigned>(order_key(v, 0) >> 32); }
 
+__device__ __forceinline__ unsigned wave_max_u(unsigned v) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        const unsigned o = __shfl_xor(v, d);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+// Largest T that at least `want` (>= 1) of the wave's N values a lane reach, or a smaller one that
+// exactly `want` reach; 0 if fewer than `want` are above 0.  `reach`: how many reach it.
+template <int N>
+__device__ __forceinline__ unsigned wave_nth(const unsigned (&v)[N], int want, int& reach) {
+    auto count = [&](unsigned t) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(v[i] >= t));
+        return c;
+    };
+    reach = count(1);
+    if (reach < want) return 0;
+    unsigned lo = 1, top = v[0], low = ~0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        top = v[i] > top ? v[i] : top;
+        low = v[i] && v[i] < low ? v[i] : low;
+    }
+    unsigned hi = wave_max_u(top);                               // hi - 1 may be T
+    const unsigned least = ~wave_max_u(~low);
+    if (least > lo) lo = least;                                  // all that are above 0 reach it
+    hi = hi == ~0u ? hi : hi + 1;
+    while (reach != want && hi - lo > 1) {
+        const unsigned mid = lo + (hi - lo) / 2;
+        const int c = count(mid);
+        if (c >= want) {
+            lo = mid;
+            reach = c;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
+}
+
+template <int THREADS>
+struct TopState {
+    uint64_t* mine;          // the wave's candidates
+    int held;                // how many were found (more than kRoom: some are lost)
+    float floor;
+    __device__ __forceinline__ void add(bool hit, uint64_t key) {
+        const uint64_t m = __ballot(hit);
+        if (!m) return;
+        const int at = held + lanes_below(m);
+        if (hit && at < TopLds<THREADS>::kRoom) mine[at] = key;
+        held += __popcll(m);
+    }
+};
+
+// A better floor; drops what is below it.  False if candidates were lost.  Two barriers.
+template <int THREADS>
+__device__ __forceinline__ bool top_raise(TopLds<THREADS>& l, TopState<THREADS>& t, int top) {
+    using L = TopLds<THREADS>;
+    constexpr int kRegs = L::kRoom / kWave;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int have = t.held < L::kRoom ? t.held : L::kRoom;
+    unsigned v[kRegs];
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) v[i] = lane + i * kWave < have ? static_cast<unsigned>(t.mine[lane + i * kWave] >> 32) : 0;
+    int reach;
+    const unsigned nth = wave_nth(v, (top + L::kWaves - 1) / L::kWaves, reach);
+    if (lane == 0) {
+        l.held[wave] = t.held;
+        l.floor[wave] = nth ? key_value(static_cast<uint64_t>(nth) << 32) : -kInf;
+    }
+    __syncthreads();
+    float floor = l.floor[0];
+    bool fits = l.held[0] <= L::kRoom;
+#pragma unroll
+    for (int w = 1; w < L::kWaves; ++w) {
+        floor = fminf(floor, l.floor[w]);
+        fits = fits && l.held[w] <= L::kRoom;
+    }
+    t.floor = fmaxf(t.floor, floor);
+    const unsigned least = order_of(t.floor);
+    int kept = 0;
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+        if (i * kWave >= have) continue;
+        const uint64_t m = __ballot(v[i] >= least && v[i]);
+        const uint64_t key = lane + i * kWave < have ? t.mine[lane + i * kWave] : 0;
+        if (m >> lane & 1) t.mine[kept + lanes_below(m)] = key;
+        kept += __popcll(m);
+    }
+    t.held = kept;
+    __syncthreads();
+    return fits;
+}
+
+// The candidates in order into l.list.  All threads; one barrier before, one after.
+template <int THREADS>
+__device__ __forceinline__ bool top_rank(TopLds<THREADS>& l, TopState<THREADS>& t, int top) {
+    using L = TopLds<THREADS>;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    if (lane == 0) l.held[wave] = t.held;
+    __syncthreads();
+    bool fits = true;
+#pragma unroll
+    for (int w = 0; w < L::kWaves; ++w) fits = fits && l.held[w] <= L::kRoom;
+    if (fits) {
+        for (int i = lane; i < t.held; i += kWave) {
+            const uint64_t key = t.mine[i];
+            int rank = 0;
+            for (int w = 0; w < L::kWaves; ++w) {
+                const int n = l.held[w];
+                const uint64_t* o = l.cand + w * L::kRoom;
+                for (int j = 0; j < n; ++j) rank += o[j] > key;
+            }
+            if (rank < top) l.list[rank] = key;
+        }
+    }
+    __syncthreads();
+    return fits;
+}
+
+// The first chunk's bound.  `best`: the caller's largest element as order_of (0: none).  Afterwards
+// l.limit is the bound (0: fewer than `top` groups have an element) and l.limit_group the last group
+// whose equal elements are needed (all of them: INT32_MAX).
+template <int THREADS>
+__device__ __forceinline__ void top_bound(TopLds<THREADS>& l, unsigned best, int top) {
+    using L = TopLds<THREADS>;
+    constexpr int kShare = THREADS / L::kGroups, kRegs = L::kGroups / kWave;
+    const int tid = threadIdx.x;
+    if (tid % kShare == 0) l.bound[tid / kShare] = best;
+    __syncthreads();
+    if (tid < kWave) {
+        unsigned v[kRegs];
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) v[i] = l.bound[i * kWave + tid];
+        int reach;
+        const unsigned nth = wave_nth(v, top, reach);
+        int group = INT32_MAX;
+        if (nth && reach > top) {                                // nth exactly, and more than needed are equal
+            int need = top;
+#pragma unroll
+            for (int i = 0; i < kRegs; ++i) need -= __popcll(__ballot(v[i] > nth));
+#pragma unroll
+            for (int i = 0; i < kRegs; ++i) {
+                const uint64_t m = __ballot(v[i] == nth);
+                const int c = __popcll(m);
+                if (group == INT32_MAX && need <= c)
+                    group = i * kWave + __ffsll(__ballot((m >> tid & 1) && lanes_below(m) == need - 1)) - 1;
+                need -= c;
+            }
+        }
+        if (tid == 0) {
+            l.limit = nth;
+            l.limit_group = group;
+            l.tie = 0;
+        }
+    }
+    __syncthreads();
+}
+
+// Steps of 8 elements per group; exact for every row, NaN included.
 template <int DT, int THREADS>
-__device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw* x, int vocab, int top, TopLds& l, TopState& t) {
-    t = {0, 0, -kInf};
+__device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw* x, int vocab, int top, TopLds<THREADS>& l) {
+    using L = TopLds<THREADS>;
+    const int tid = threadIdx.x;
+    int have = 0;
     uint64_t low = 0;                                            // the list's last key once it is full
-    __syncthreads();
-    if (threadIdx.x == 0) l.count = 0;
-    __syncthreads();
-    constexpr int kStep = kGroups * 8;
+    constexpr int kStep = L::kGroups * 8;
     for (int base = 0; base < vocab; base += kStep) {
+        __syncthreads();
+        if (tid == 0) l.count = 0;
         uint64_t best = 0;
         uint64_t keys[8];
+#pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int i = base + static_cast<int>(threadIdx.x) * 8 + j;
-            const bool in = threadIdx.x < kGroups && i < vocab;
+            const int i = base + tid * 8 + j;
+            const bool in = tid < L::kGroups && i < vocab;
             keys[j] = in ? order_key(Elem<DT>::widen(x[i]), i) : 0;
             if (keys[j] <= low) keys[j] = 0;
             best = keys[j] > best ? keys[j] : best;
         }
         // keys are all different, so at most 8 * top elements reach the top-th of the groups' best
-        if (threadIdx.x < kGroups) l.cand[threadIdx.x] = best;
-        if (threadIdx.x == 0) l.limit = 0;
+        if (tid < L::kGroups) l.cand[tid] = best;
+        if (tid == 0) l.reach = 0;
         __syncthreads();
-        if (threadIdx.x < kGroups && best) {
+        if (tid < L::kGroups && best) {
             int rank = 0;
-            for (int j = 0; j < kGroups; ++j) rank += l.cand[j] > best;
-            if (rank == top - 1) l.limit = best;
+            for (int j = 0; j < L::kGroups; ++j) rank += l.cand[j] > best;
+            if (rank == top - 1) l.reach = best;
         }
         __syncthreads();
-        const uint64_t limit = l.limit;
-        __syncthreads();
+        const uint64_t reach = l.reach;
+#pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (keys[j] && keys[j] >= limit) top_push(l, keys[j]);
-        top_refresh<THREADS>(l, t, top);
-        if (t.have == top) low = l.list[t.side][top - 1];
+            if (keys[j] && keys[j] >= reach) l.cand[atomicAdd(&l.count, 1u)] = keys[j];
+        __syncthreads();
+        const int n = static_cast<int>(l.count), total = have + n;
+        constexpr int kOwn = (8 * L::kGroups + L::kGroups + THREADS - 1) / THREADS;
+        uint64_t own[kOwn];
+        int rank[kOwn];
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) {
+            const int i = tid + e * THREADS;
+            own[e] = 0;
+            rank[e] = top;
+            if (i >= total) continue;
+            own[e] = i < have ? l.list[i] : l.cand[i - have];
+            rank[e] = 0;
+            for (int j = 0; j < have; ++j) rank[e] += l.list[j] > own[e];
+            for (int j = 0; j < n; ++j) rank[e] += l.cand[j] > own[e];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e)
+            if (rank[e] < top) l.list[rank[e]] = own[e];
+        __syncthreads();
+        have = total < top ? total : top;
+        if (have == top) low = l.list[top - 1];
     }
+    __syncthreads();
 }
 
 struct ScoreArgs {
@@ -405,13 +551,17 @@ __device__ __forceinline__ float log_prob(const RowStat& st, const Scale& sc, fl
 // while one is summed.
 constexpr int kU = 4;
 
+// Blocks of 256 threads: eight fit a CU by their LDS (19.6 KiB), 64 registers a thread.
+constexpr int scores_waves(int threads, bool top) { return !top ? 1 : threads == 1024 ? 4 : threads == 256 ? 8 : 6; }
+
 template <int DT, int THREADS, bool TOP>
-__global__ __launch_bounds__(THREADS) void token_scores_kernel(const ScoreArgs a) {
+__global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_scores_kernel(const ScoreArgs a) {
     using E = Elem<DT>;
     using V = Vec<DT>;
+    using L = TopLds<THREADS>;
     __shared__ Acc lds[THREADS / kWave];
     __shared__ float red[THREADS / kWave];
-    __shared__ TopLds l;
+    __shared__ L l;
     const int64_t row = blockIdx.x;
     const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
     const Span sp = V::span(x, a.vocab);
@@ -419,80 +569,60 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(const ScoreArgs a
     const int tid = threadIdx.x;
     const float k = a.scale.k;
     Acc acc = acc_empty();
-    TopState t = {0, 0, -kInf};
-    bool lost = false;
-    if (TOP && tid == 0) l.count = 0;
+    TopState<THREADS> t = {l.cand + (tid / kWave) * L::kRoom, 0, -kInf};
 
-    uint4 next[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-        const int i = u * THREADS + tid;
-        next[u] = i < sp.nvec ? load_once(body + i) : V::fill();
-    }
-    // one element of the row's ends per thread: head elements belong to the first chunk
-    const float head = tid < sp.head ? E::widen(x[tid]) : -kInf;
-    const float tail = tid < sp.tail ? E::widen(x[a.vocab - sp.tail + tid]) : -kInf;
-
-    int due = 1;                                                 // chunks read at the next refresh
-    int chunk = 0;
-    for (int base = 0; base < sp.nvec || chunk == 0; ++chunk) {
-        uint4 cur[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) cur[u] = next[u];
-        const int first = base;
-        base += kU * THREADS;
-        if (base < sp.nvec) {
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int i = base + u * THREADS + tid;
-                next[u] = i < sp.nvec ? load_once(body + i) : V::fill();
-            }
-        }
-        float v[kU * V::N];
+    uint4 cur[kU], next[kU];
+    auto fetch = [&](int base) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            float w[V::N];
-            V::widen(cur[u], w);
-#pragma unroll
-            for (int i = 0; i < V::N; ++i) v[u * V::N + i] = w[i];
+            const int i = base + u * THREADS + tid;
+            next[u] = i < sp.nvec ? load_once(body + i) : V::fill();
         }
-        float peak = v[0];
+    };
+    fetch(0);
+    // the row's ends, an element a thread: the head belongs to the first chunk, the tail behind the last
+    const float head = tid < sp.head ? E::widen(x[tid]) : -kInf;
+    const float tail = tid < sp.tail ? E::widen(x[a.vocab - sp.tail + tid]) : -kInf;
 #pragma unroll
-        for (int i = 1; i < kU * V::N; ++i) peak = fmaxf(peak, v[i]);
-        if (chunk == 0) {
-            const float ends = fmaxf(head, tail);
-            acc_raise<true>(acc, fmaxf(acc.R, fminf(rintf(ends * k), kFar)));
-            acc_one<true>(acc, head, k);
-            acc_one<true>(acc, tail, k);
-        }
+    for (int u = 0; u < kU; ++u) cur[u] = next[u];
+    if (kU * THREADS < sp.nvec) fetch(kU * THREADS);
+    {
+        const float v[2] = {head, tail};
+        acc_add<true>(acc, v, fmaxf(head, tail), k);
+    }
+    float most = head;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+        float v[V::N];
+        V::widen(cur[u], v);
+        const float peak = max_of(v);
+        most = fmaxf(most, peak);
         acc_add<true>(acc, v, peak, k);
-        if (!TOP) continue;
-        if (chunk == 0) {
-            // the bound: groups of threads (one each, or four neighbours of 1024)
-            const float top0 = fmaxf(peak, head);
-            const bool any = tid < sp.head || tid < sp.nvec;
-            unsigned mine = any ? order_of(top0) : 0;
-            constexpr int kShare = THREADS / kGroups;
-            for (int d = 1; d < kShare; d <<= 1) {
-                const unsigned o = __shfl_xor(mine, d);
-                mine = o > mine ? o : mine;
-            }
-            if (tid == 0) l.tie = 0;
-            const uint64_t limit = top_bound<THREADS>(l, mine, tid / kShare, tid % kShare == 0, a.top);
-            const float lim = limit ? key_value(limit) : -kInf;
-            const unsigned valid = low_bits(V::N * (tid < sp.nvec ? (sp.nvec - 1 - tid) / THREADS + 1 : 0));
-            const int place = sp.head + tid * V::N;
-            unsigned above = 0, equal = 0;
+    }
+    if (TOP) {
+        constexpr int kShare = THREADS / L::kGroups;
+        unsigned best = tid < sp.head || tid < sp.nvec ? order_of(most) : 0;
+        for (int d = 1; d < kShare; d <<= 1) {
+            const unsigned o = __shfl_xor(best, d);
+            best = o > best ? o : best;
+        }
+        top_bound(l, best, a.top);
+        const unsigned limit = l.limit, last = l.limit_group;
+        const float lim = limit ? key_value(static_cast<uint64_t>(limit) << 32) : -kInf;
+        int tie = INT32_MAX;
+        if (last != INT32_MAX) {
+            // groups up to `last` at the bound's value: the lowest index of each has to be let in
+            if (best == limit && static_cast<unsigned>(tid / kShare) <= last) {
+                int at = tid < sp.head && head == lim ? tid : INT32_MAX;
 #pragma unroll
-            for (int i = 0; i < kU * V::N; ++i) {
-                above |= static_cast<unsigned>(v[i] > lim) << i;
-                equal |= static_cast<unsigned>(v[i] == lim) << i;
-            }
-            above &= valid;
-            equal &= valid;
-            if (limit && static_cast<unsigned>(limit >> 32) == mine && static_cast<unsigned>(tid / kShare) <= key_index(limit)) {
-                // the groups at the bound's value: the lowest index of each has to be let in
-                int at = tid < sp.head && head == lim ? tid : equal ? chunk_index<THREADS, V::N>(place, equal) : INT32_MAX;
+                for (int u = 0; u < kU; ++u) {
+                    float v[V::N];
+                    V::widen_again(cur[u], v);
+#pragma unroll
+                    for (int i = 0; i < V::N; ++i)
+                        if (at == INT32_MAX && u * THREADS + tid < sp.nvec && v[i] == lim)
+                            at = sp.head + (u * THREADS + tid) * V::N + i;
+                }
                 for (int d = 1; d < kShare; d <<= 1) {
                     const int o = __shfl_xor(at, d);
                     at = o < at ? o : at;
@@ -500,33 +630,53 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(const ScoreArgs a
                 atomicMax(&l.tie, static_cast<unsigned>(at));
             }
             __syncthreads();
-            const int tie = limit ? static_cast<int>(l.tie) : INT32_MAX;
-            if (tid < sp.head && (head > lim || (head == lim && tid <= tie))) top_push(l, order_key(head, tid));
-            for (unsigned m = above | equal; m; m &= m - 1) {
-                const int at = chunk_index<THREADS, V::N>(place, m);
-                const float w = E::widen(x[at]);
-                if (w > lim || at <= tie) top_push(l, order_key(w, at));
-            }
-        } else if (peak > t.floor) {
-            unsigned above = 0;
+            tie = static_cast<int>(l.tie);
+        }
+        t.add(tid < sp.head && (head > lim || (head == lim && tid <= tie)), order_key(head, tid));
 #pragma unroll
-            for (int i = 0; i < kU * V::N; ++i) above |= static_cast<unsigned>(v[i] > t.floor) << i;
-            const int place = sp.head + (first + tid) * V::N;
-            for (; above; above &= above - 1) {                  // few: read again rather than picked from registers
-                const int at = chunk_index<THREADS, V::N>(place, above);
-                top_push(l, order_key(E::widen(x[at]), at));
+        for (int u = 0; u < kU; ++u) {
+            float v[V::N];
+            V::widen_again(cur[u], v);
+            const bool in = u * THREADS + tid < sp.nvec;
+            if (!__any(in && max_of(v) >= lim)) continue;
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) {
+                const int at = sp.head + (u * THREADS + tid) * V::N + i;
+                t.add(in && (v[i] > lim || (v[i] == lim && at <= tie)), order_key(v[i], at));
             }
         }
-        if (chunk + 1 == due && base < sp.nvec) {
-            if (!lost) lost = !top_refresh<THREADS>(l, t, a.top);
+        t.floor = lim;           // `top` elements reach it; -inf without a bound, and there is no further chunk
+    }
+    bool fits = true;
+    int chunk = 1, due = 2;                                      // chunks read when the floor is raised next
+    for (int base = kU * THREADS; base < sp.nvec; ++chunk) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) cur[u] = next[u];
+        const int first = base;
+        base += kU * THREADS;
+        if (base < sp.nvec) fetch(base);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float v[V::N];
+            V::widen(cur[u], v);
+            const float peak = max_of(v);
+            acc_add<true>(acc, v, peak, k);
+            if (TOP && __any(peak > t.floor)) {
+#pragma unroll
+                for (int i = 0; i < V::N; ++i)
+                    t.add(v[i] > t.floor, order_key(v[i], sp.head + (first + u * THREADS + tid) * V::N + i));
+            }
+        }
+        if (TOP && chunk + 1 == due && base < sp.nvec) {
+            fits = top_raise(l, t, a.top) && fits;
             due *= 2;
         }
     }
     if (TOP) {
-        // the last elements; before the first refresh (a row of one chunk) all of them are candidates
-        if (tid < sp.tail && (t.have < a.top || tail > t.floor))
-            top_push(l, order_key(tail, a.vocab - sp.tail + tid));
-        if (!lost) lost = !top_refresh<THREADS>(l, t, a.top);
+        // without a bound every element is a candidate
+        t.add(tid < sp.tail && (l.limit == 0 || tail > t.floor), order_key(tail, a.vocab - sp.tail + tid));
+        if (chunk > 1) fits = top_raise(l, t, a.top) && fits;
+        fits = top_rank(l, t, a.top) && fits;
     }
     acc = acc_block<true, THREADS>(acc, lds);
     RowStat st = {acc.R, acc.s, 0.0f, log2f(acc.s), 0.0f, false};
@@ -535,9 +685,9 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(const ScoreArgs a
     if (!acc_good(acc)) {
         st = slow_stat<DT, THREADS>(x, a.vocab, a.scale.inv_tau, red);
         lse = st.m + st.log_s;
-        lost = true;
+        fits = false;
     }
-    if (TOP && lost) slow_top<DT, THREADS>(x, a.vocab, a.top, l, t);
+    if (TOP && !fits) slow_top<DT, THREADS>(x, a.vocab, a.top, l);
     if (tid == 0) {
         a.lse[row] = lse;
         a.entropy[row] = st.entropy;
@@ -551,9 +701,10 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(const ScoreArgs a
     }
     if (TOP) {
         for (int j = tid; j < a.top; j += THREADS) {
-            const uint64_t key = l.list[t.side][j];
+            const uint64_t key = l.list[j];
+            const float v = static_cast<unsigned>(key >> 32) == 0xfffffffeu ? __builtin_nanf("") : key_value(key);
             a.top_ids[row * a.top + j] = static_cast<int32_t>(key_index(key));
-            a.top_logprobs[row * a.top + j] = log_prob(st, a.scale, E::widen(x[key_index(key)]), lse);
+            a.top_logprobs[row * a.top + j] = log_prob(st, a.scale, v, lse);
         }
     }
 }
@@ -827,10 +978,7 @@ __device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int voca
                 next[u] = i < sp.nvec ? body[i] : V::fill();
             }
         }
-        float peak = v[0];
-#pragma unroll
-        for (int i = 1; i < kU * V::N; ++i) peak = fmaxf(peak, v[i]);
-        acc_add<false>(acc, v, peak, k);
+        acc_add<false>(acc, v, max_of(v), k);
     }
     return acc;
 }
@@ -1221,7 +1369,10 @@ void launch_scores_t(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
 
 template <int DT>
 void launch_scores(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
-    if (wide_blocks(x->outer * x->inner, x->vocab))
+    // a short row is one wave's: no barriers (its first chunk bounds up to 64 entries)
+    if (x->vocab <= 4096 && a.top <= kWave / 2)
+        launch_scores_t<DT, kWave>(x, a, st);
+    else if (wide_blocks(x->outer * x->inner, x->vocab))
         launch_scores_t<DT, 1024>(x, a, st);
     else
         launch_scores_t<DT, 256>(x, a, st);
