@@ -50,6 +50,14 @@ struct Rows {            // a [outer, inner, vocab] view with unit stride along 
     }
 };
 
+template <int N>
+__device__ __forceinline__ float max_of(const float (&v)[N]) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+    return m;
+}
+
 // 16 bytes of a row, and the rest of it: `head` elements before the first 16-byte boundary, `nvec`
 // vectors, `tail` elements behind the last one.
 struct Span {
@@ -88,6 +96,19 @@ struct Vec {
             }
         }
     }
+    // The largest element; for float16 by pairs, so that the conversion is left to the multiply-add.
+    static __device__ __forceinline__ float peak(const uint4& r, const float (&v)[N]) {
+        if constexpr (DT == FA_LOGITS_F16) {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            const h2 m = __builtin_elementwise_max(
+                __builtin_elementwise_max(__builtin_bit_cast(h2, r.x), __builtin_bit_cast(h2, r.y)),
+                __builtin_elementwise_max(__builtin_bit_cast(h2, r.z), __builtin_bit_cast(h2, r.w)));
+            const _Float16 lo = m.x, hi = m.y;
+            return fmaxf(static_cast<float>(lo), static_cast<float>(hi));
+        } else {
+            return max_of(v);
+        }
+    }
     // The same for a value that was widened before: costs less than the registers to keep it.
     static __device__ __forceinline__ void widen_again(uint4 r, float (&v)[N]) {
         asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
@@ -105,14 +126,6 @@ struct Vec {
         return {w[0], w[1], w[2], w[3]};
     }
 };
-
-template <int N>
-__device__ __forceinline__ float max_of(const float (&v)[N]) {
-    float m = v[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-    return m;
-}
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -278,7 +291,7 @@ __device__ __forceinline__ float key_value(uint64_t key) {       // not for a Na
 // elements reach, and the elements that reach it become candidates, in a buffer of their wave.  From
 // then on only elements above the floor -- a value that `top` elements before them reach -- are
 // candidates (an equal one has a higher index), found by comparing the largest of a vector's elements.
-// The floor is raised after chunks 1, 3, 7, ... and at the end: with W waves, the least of the waves'
+// The floor is raised when 4, 8, 16, ... chunks have been read (2, 4, 8, ... cost 3 % more at 2048 x 50261) and at the end: with W waves, the least of the waves'
 // ceil(top / W)-th largest candidates.  Candidates below it are dropped; in a row in no particular
 // order about top * (1 + ln(n / chunk)) elements ever become candidates.  The last ones are ranked
 // against each other.
@@ -373,8 +386,15 @@ __device__ __forceinline__ bool top_raise(TopLds<THREADS>& l, TopState<THREADS>&
     unsigned v[kRegs];
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) v[i] = lane + i * kWave < have ? static_cast<unsigned>(t.mine[lane + i * kWave] >> 32) : 0;
+    const int want = (top + L::kWaves - 1) / L::kWaves;
     int reach;
-    const unsigned nth = wave_nth(v, (top + L::kWaves - 1) / L::kWaves, reach);
+    unsigned nth;
+    if (have <= kWave) {                                         // the usual case in one register
+        const unsigned one[1] = {v[0]};
+        nth = wave_nth(one, want, reach);
+    } else {
+        nth = wave_nth(v, want, reach);
+    }
     if (lane == 0) {
         l.held[wave] = t.held;
         l.floor[wave] = nth ? key_value(static_cast<uint64_t>(nth) << 32) : -kInf;
@@ -409,6 +429,9 @@ __device__ __forceinline__ bool top_rank(TopLds<THREADS>& l, TopState<THREADS>& 
     using L = TopLds<THREADS>;
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     if (lane == 0) l.held[wave] = t.held;
+    // zeros, which rank below every key, up to a multiple of kStep
+    constexpr int kStep = 8;
+    if (lane < kStep && t.held + lane < (t.held + kStep - 1) / kStep * kStep && t.held + lane < L::kRoom) t.mine[t.held + lane] = 0;
     __syncthreads();
     bool fits = true;
 #pragma unroll
@@ -420,7 +443,13 @@ __device__ __forceinline__ bool top_rank(TopLds<THREADS>& l, TopState<THREADS>& 
             for (int w = 0; w < L::kWaves; ++w) {
                 const int n = l.held[w];
                 const uint64_t* o = l.cand + w * L::kRoom;
-                for (int j = 0; j < n; ++j) rank += o[j] > key;
+                for (int j = 0; j < n; j += kStep) {             // kStep reads on their way at once
+                    uint64_t other[kStep];
+#pragma unroll
+                    for (int q = 0; q < kStep; ++q) other[q] = o[j + q];
+#pragma unroll
+                    for (int q = 0; q < kStep; ++q) rank += other[q] > key;
+                }
             }
             if (rank < top) l.list[rank] = key;
         }
@@ -595,7 +624,7 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
     for (int u = 0; u < kU; ++u) {
         float v[V::N];
         V::widen(cur[u], v);
-        const float peak = max_of(v);
+        const float peak = V::peak(cur[u], v);
         most = fmaxf(most, peak);
         acc_add<true>(acc, v, peak, k);
     }
@@ -648,7 +677,14 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
         t.floor = lim;           // `top` elements reach it; -inf without a bound, and there is no further chunk
     }
     bool fits = true;
-    int chunk = 1, due = 2;                                      // chunks read when the floor is raised next
+    // Chunks read when the floor is raised next.  The first chunk's bound is near the top-th element
+    // while `top` is well below the number of groups; beyond three quarters of it a wave's room would
+    // not last four chunks.
+    int chunk = 1, due = 4;
+    if (TOP && a.top > L::kGroups * 3 / 4) {
+        fits = top_raise(l, t, a.top);
+        due = 2;
+    }
     for (int base = kU * THREADS; base < sp.nvec; ++chunk) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) cur[u] = next[u];
@@ -659,7 +695,7 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
         for (int u = 0; u < kU; ++u) {
             float v[V::N];
             V::widen(cur[u], v);
-            const float peak = max_of(v);
+            const float peak = V::peak(cur[u], v);
             acc_add<true>(acc, v, peak, k);
             if (TOP && __any(peak > t.floor)) {
 #pragma unroll
@@ -962,14 +998,9 @@ __device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int voca
         next[u] = i < sp.nvec ? body[i] : V::fill();
     }
     for (int base = 0; base < sp.nvec;) {
-        float v[kU * V::N];
+        uint4 cur[kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            float w[V::N];
-            V::widen(next[u], w);
-#pragma unroll
-            for (int i = 0; i < V::N; ++i) v[u * V::N + i] = w[i];
-        }
+        for (int u = 0; u < kU; ++u) cur[u] = next[u];
         base += kU * THREADS;
         if (base < sp.nvec) {
 #pragma unroll
@@ -978,7 +1009,12 @@ __device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int voca
                 next[u] = i < sp.nvec ? body[i] : V::fill();
             }
         }
-        acc_add<false>(acc, v, max_of(v), k);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float v[V::N];
+            V::widen(cur[u], v);
+            acc_add<false>(acc, v, V::peak(cur[u], v), k);
+        }
     }
     return acc;
 }
