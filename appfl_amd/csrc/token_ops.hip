@@ -135,6 +135,11 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
     return {v.x, v.y, v.z, v.w};
 }
 
+__device__ __forceinline__ void store_once(uint4* p, const uint4& r) {
+    const u32x4 v = {r.x, r.y, r.z, r.w};
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p));
+}
+
 // ---- softmax statistics ---------------------------------------------------------------------------
 // With k = log2(e) / T every term is 2^(x k - R), R a whole number near the largest x k: the
 // multiply-add rounds once, relative to its small result, rescaling by a power of two is exact, and
@@ -780,7 +785,8 @@ struct TeacherLds {
 };
 
 struct Teacher {
-    float t[kPer], log_t[kPer], x[kPer];
+    int id[kPer];
+    float lp[kPer], t[kPer], log_t[kPer], x[kPer];
 };
 
 __device__ __forceinline__ float wave_max_f(float v) {
@@ -795,28 +801,38 @@ __device__ __forceinline__ float wave_sum_f(float v) {
     return v;
 }
 
+// In three steps, so that a kernel can put its own loads between them.
+__device__ __forceinline__ void teacher_fetch(const TeacherArgs& a, int64_t row, Teacher& r) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int j = threadIdx.x + kWave * i;
+        r.id[i] = -1;
+        r.lp[i] = -kInf;
+        if (j < a.k) {
+            r.id[i] = a.ids[row * a.id_stride + j];
+            r.lp[i] = a.lp[row * a.lp_stride + j];
+        }
+    }
+}
+
 template <int DT>
-__device__ __forceinline__ Teacher teacher_row(const TeacherArgs& a, int64_t row, const typename Elem<DT>::Raw* x, int vocab,
-                                               float inv_tau, TeacherLds& l) {
+__device__ __forceinline__ void teacher_gather(const typename Elem<DT>::Raw* x, int vocab, Teacher& r) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        r.x[i] = -kInf;
+        if (r.id[i] >= 0 && r.id[i] < vocab) r.x[i] = Elem<DT>::widen(x[r.id[i]]);
+    }
+}
+
+__device__ __forceinline__ void teacher_make(Teacher& r, int vocab, float inv_tau, TeacherLds& l) {
     const int lane = threadIdx.x;
-    Teacher r;
-    int id[kPer];
-    float lp[kPer];
     bool bad = false;
     float peak = -kInf;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int j = lane + kWave * i;
-        id[i] = -1;
-        lp[i] = -kInf;
-        r.x[i] = -kInf;
-        if (j < a.k) {
-            id[i] = a.ids[row * a.id_stride + j];
-            if (id[i] >= 0) lp[i] = a.lp[row * a.lp_stride + j];
-            if (id[i] >= 0 && id[i] < vocab) r.x[i] = Elem<DT>::widen(x[id[i]]);
-        }
-        bad = bad || id[i] >= vocab || lp[i] != lp[i] || lp[i] == kInf;
-        peak = fmaxf(peak, lp[i]);
+        if (r.id[i] < 0) r.lp[i] = -kInf;
+        bad = bad || r.id[i] >= vocab || r.lp[i] != r.lp[i] || r.lp[i] == kInf;
+        peak = fmaxf(peak, r.lp[i]);
     }
     bad = __any(bad);
     peak = wave_max_f(peak);
@@ -824,7 +840,7 @@ __device__ __forceinline__ Teacher teacher_row(const TeacherArgs& a, int64_t row
     float z = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        r.log_t[i] = lp[i] == -kInf ? -kInf : (lp[i] - peak) * inv_tau;
+        r.log_t[i] = r.lp[i] == -kInf ? -kInf : (r.lp[i] - peak) * inv_tau;
         r.t[i] = exp2_hw(r.log_t[i] * kLog2e);
         z += r.t[i];
     }
@@ -835,17 +851,14 @@ __device__ __forceinline__ Teacher teacher_row(const TeacherArgs& a, int64_t row
         const int j = lane + kWave * i;
         r.log_t[i] -= log_z;
         r.t[i] = empty ? 0.0f : r.t[i] * inv_z;
-        if (j < FA_TOP_MAX) {
-            l.id[j] = id[i] < vocab ? id[i] : -1;
-            l.t[j] = r.t[i];
-            l.x[j] = r.x[i];
-        }
+        l.id[j] = r.id[i] < vocab ? r.id[i] : -1;
+        l.t[j] = r.t[i];
+        l.x[j] = r.x[i];
     }
     if (lane == 0) {
         l.empty = empty;
         l.bad = bad;
     }
-    return r;
 }
 
 // Entries that name one token: the first takes their probabilities together (the gradient's term).
@@ -925,7 +938,8 @@ __device__ __forceinline__ Softmax softmax_of(const RowStat& st, const Scale& sc
 
 // Writes f(element) over elements [lo, hi) of a row; reads by 16 bytes, writes so where the
 // gradient's row has the same alignment.
-template <int DT, int THREADS, class F>
+// LAST: the elements are read past the caches.
+template <int DT, int THREADS, bool LAST, class F>
 __device__ __forceinline__ void map_row(const typename Elem<DT>::Raw* x, typename Elem<DT>::Raw* g, int vocab, int part,
                                         int parts, F f) {
     using E = Elem<DT>;
@@ -946,7 +960,7 @@ __device__ __forceinline__ void map_row(const typename Elem<DT>::Raw* x, typenam
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int i = base + u * THREADS + tid;
-            if (i < hi) r[u] = body[i];
+            if (i < hi) r[u] = LAST ? load_once(body + i) : body[i];
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
@@ -957,7 +971,7 @@ __device__ __forceinline__ void map_row(const typename Elem<DT>::Raw* x, typenam
 #pragma unroll
             for (int j = 0; j < V::N; ++j) v[j] = f(v[j]);
             if (same) {
-                reinterpret_cast<uint4*>(g + sp.head)[i] = V::narrow(v);
+                store_once(reinterpret_cast<uint4*>(g + sp.head) + i, V::narrow(v));
             } else {
 #pragma unroll
                 for (int j = 0; j < V::N; ++j) g[sp.head + i * V::N + j] = E::narrow(v[j]);
@@ -1019,7 +1033,10 @@ __device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int voca
     return acc;
 }
 
-template <int DT, int THREADS, bool LOSS, bool GRAD>
+// LOSS alone: the sums of a row.  GRAD alone: from the sums of an earlier call; a row may be cut in
+// parts (blockIdx.y).  Both: the row is read twice, the second time from the memory-side cache as long
+// as the rows under way fit there (see step_threads).
+template <int DT, int THREADS, bool LOSS, bool GRAD, bool LAST>
 __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     using E = Elem<DT>;
     __shared__ Acc lds[THREADS / kWave];
@@ -1033,7 +1050,9 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     const bool first_wave = threadIdx.x < kWave;
     Teacher e;
     if (first_wave) {
-        e = teacher_row<DT>(a.t, row, x, a.vocab, a.scale.inv_tau, l);
+        teacher_fetch(a.t, row, e);
+        teacher_gather<DT>(x, a.vocab, e);
+        teacher_make(e, a.vocab, a.scale.inv_tau, l);
         if (GRAD) teacher_unite(a.t.k, l);
     }
     RowStat st;
@@ -1068,11 +1087,11 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     typename E::Raw* g = static_cast<typename E::Raw*>(a.grad) + a.grad_rows.offset(row);
     if (off || c == 0.0f || l.bad) {
         const float v = !off && l.bad ? __builtin_nanf("") : 0.0f;
-        map_row<DT, THREADS>(x, g, a.vocab, part, parts, [v](float) { return v; });
+        map_row<DT, THREADS, LAST>(x, g, a.vocab, part, parts, [v](float) { return v; });
         return;
     }
     const Softmax f = softmax_of(st, a.scale, c);
-    map_row<DT, THREADS>(x, g, a.vocab, part, parts, f);
+    map_row<DT, THREADS, LAST>(x, g, a.vocab, part, parts, f);
     __syncthreads();
     if (first_wave) {
         const Span sp = Vec<DT>::span(x, a.vocab);
@@ -1080,6 +1099,92 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
         const int hi = part == parts - 1 ? a.vocab : sp.head + static_cast<int>(static_cast<int64_t>(sp.nvec) * (part + 1) / parts) * Vec<DT>::N;
         fix_row<DT>(g, l, a.t.k, lo, hi, f);
     }
+}
+
+// Loss and gradient of a row that stays in its block's registers between the sums and the gradient:
+// read once, written once.  NV vectors of 16 bytes a thread.
+template <int DT, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void distill_step_kernel(const DistillArgs a) {
+    using E = Elem<DT>;
+    using V = Vec<DT>;
+    __shared__ Acc lds[THREADS / kWave];
+    __shared__ float red[THREADS / kWave];
+    __shared__ TeacherLds l;
+    const int64_t row = blockIdx.x;
+    const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
+    typename E::Raw* g = static_cast<typename E::Raw*>(a.grad) + a.grad_rows.offset(row);
+    const float weight = a.t.row_weight ? a.t.row_weight[row] : 1.0f;
+    const float c = weight * a.t.tau;
+    const bool first_wave = threadIdx.x < kWave;
+    const int tid = threadIdx.x;
+    const Span sp = V::span(x, a.vocab);
+    const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
+    const float k = a.scale.k;
+    Teacher e;
+    if (first_wave) teacher_fetch(a.t, row, e);
+    uint4 r[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int i = u * THREADS + tid;
+        r[u] = i < sp.nvec ? load_once(body + i) : V::fill();
+    }
+    const bool has_head = tid < sp.head, has_tail = tid < sp.tail;
+    const int tail_at = a.vocab - sp.tail + tid;
+    const float head = has_head ? E::widen(x[tid]) : -kInf, tail = has_tail ? E::widen(x[tail_at]) : -kInf;
+    if (first_wave) teacher_gather<DT>(x, a.vocab, e);
+    Acc acc = acc_empty();
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        float v[V::N];
+        V::widen(r[u], v);
+        acc_add<false>(acc, v, V::peak(r[u], v), k);
+    }
+    {
+        const float v[2] = {head, tail};
+        acc_add<false>(acc, v, fmaxf(head, tail), k);
+    }
+    if (first_wave) {
+        teacher_make(e, a.vocab, a.scale.inv_tau, l);
+        teacher_unite(a.t.k, l);
+    }
+    acc = acc_block<false, THREADS>(acc, lds);
+    const bool off = weight == 0.0f || l.empty;
+    RowStat st = {acc.R, acc.s, 0.0f, log2f(acc.s), 0.0f, false};
+    if (!off && !acc_good(acc)) st = slow_stat<DT, THREADS>(x, a.vocab, a.scale.inv_tau, red);
+    if (first_wave) {
+        const float loss = off ? 0.0f : row_loss(a, e, st, weight, l.bad);
+        if (tid == 0) a.loss[row] = loss;
+    }
+    const bool flat = off || c == 0.0f || l.bad;                 // one value for the whole row
+    const float level = !off && l.bad ? __builtin_nanf("") : 0.0f;
+    const Softmax f = softmax_of(st, a.scale, c);
+    const bool same = reinterpret_cast<uintptr_t>(x) % 16 == reinterpret_cast<uintptr_t>(g) % 16;
+    uint4* out = reinterpret_cast<uint4*>(g + sp.head);
+    if (has_head) g[tid] = E::narrow(flat ? level : f(head));
+    if (has_tail) g[tail_at] = E::narrow(flat ? level : f(tail));
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int i = u * THREADS + tid;
+        if (i >= sp.nvec) continue;
+        float v[V::N];
+        V::widen_again(r[u], v);
+        if (flat) {
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) v[j] = level;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) v[j] = f(v[j]);
+        }
+        if (same) {
+            store_once(out + i, V::narrow(v));
+        } else {
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) g[sp.head + i * V::N + j] = E::narrow(v[j]);
+        }
+    }
+    if (flat) return;
+    __syncthreads();
+    if (first_wave) fix_row<DT>(g, l, a.t.k, 0, a.vocab, f);
 }
 
 // ---- merging the clients' lists -------------------------------------------------------------------
@@ -1370,28 +1475,53 @@ DistillArgs distill_args(const fa_logits* x, const fa_teacher* t) {
 // Few long rows: one block of 1024 threads each; else 256.
 bool wide_blocks(int64_t rows, int vocab) { return rows < 512 && vocab >= 8192; }
 
-template <int DT, bool LOSS, bool GRAD>
-void launch_distill_t(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
-    const int64_t rows = x->outer * x->inner;
-    int parts = 1;
-    if (!LOSS) {                 // a gradient alone has nothing to sum: a row may be cut
-        while (parts < 64 && rows * parts < 2048 && x->vocab / parts >= 8192) parts *= 2;
-    }
-    const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(parts));
-    if (LOSS && wide_blocks(rows, x->vocab))
-        hipLaunchKernelGGL((distill_kernel<DT, 1024, LOSS, GRAD>), grid, dim3(1024), 0, st, a);
-    else
-        hipLaunchKernelGGL((distill_kernel<DT, 256, LOSS, GRAD>), grid, dim3(256), 0, st, a);
+constexpr int64_t kMemoryCache = 256ll << 20;      // the last-level cache of the memory side
+
+int64_t row_bytes(const fa_logits* x) { return static_cast<int64_t>(x->vocab) * elem_size(x->dtype); }
+
+template <int DT, int THREADS, bool LOSS, bool GRAD, bool LAST>
+void launch_distill_t(int64_t rows, int parts, const DistillArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((distill_kernel<DT, THREADS, LOSS, GRAD, LAST>),
+                       dim3(static_cast<unsigned>(rows), static_cast<unsigned>(parts)), dim3(THREADS), 0, st, a);
 }
 
-template <bool LOSS, bool GRAD>
-int launch_distill(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
-    switch (x->dtype) {
-        case FA_LOGITS_F32: launch_distill_t<FA_LOGITS_F32, LOSS, GRAD>(x, a, st); break;
-        case FA_LOGITS_BF16: launch_distill_t<FA_LOGITS_BF16, LOSS, GRAD>(x, a, st); break;
-        default: launch_distill_t<FA_LOGITS_F16, LOSS, GRAD>(x, a, st);
+template <int DT>
+void launch_loss(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
+    const int64_t rows = x->outer * x->inner;
+    if (x->vocab <= 4096) launch_distill_t<DT, 64, true, false, false>(rows, 1, a, st);
+    else if (wide_blocks(rows, x->vocab)) launch_distill_t<DT, 1024, true, false, false>(rows, 1, a, st);
+    else launch_distill_t<DT, 256, true, false, false>(rows, 1, a, st);
+}
+
+// A gradient alone has nothing to sum, so that a row may be cut when there are few.
+template <int DT>
+void launch_grad(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
+    const int64_t rows = x->outer * x->inner;
+    int parts = 1;
+    while (parts < 64 && rows * parts < 2048 && x->vocab / parts >= 8192) parts *= 2;
+    if (x->vocab <= 4096) launch_distill_t<DT, 64, false, true, false>(rows, 1, a, st);
+    else launch_distill_t<DT, 256, false, true, false>(rows, parts, a, st);
+}
+
+template <int DT, int NV>
+void launch_step_t(int64_t rows, const DistillArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((distill_step_kernel<DT, kWave, NV>), dim3(static_cast<unsigned>(rows)), dim3(kWave), 0, st, a);
+}
+
+template <int DT>
+void launch_step(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
+    const int64_t rows = x->outer * x->inner;
+    const int nvec = x->vocab / Vec<DT>::N;
+    if (nvec <= kWave * 4) return launch_step_t<DT, 4>(rows, a, st);
+    if (nvec <= kWave * 8) return launch_step_t<DT, 8>(rows, a, st);
+    const bool last = rows * row_bytes(x) > kMemoryCache;
+    if (wide_blocks(rows, x->vocab) || row_bytes(x) > (128 << 10)) {
+        if (last) launch_distill_t<DT, 1024, true, true, true>(rows, 1, a, st);
+        else launch_distill_t<DT, 1024, true, true, false>(rows, 1, a, st);
+    } else {
+        if (last) launch_distill_t<DT, 256, true, true, true>(rows, 1, a, st);
+        else launch_distill_t<DT, 256, true, true, false>(rows, 1, a, st);
     }
-    return hip_code(hipGetLastError());
 }
 
 template <int DT, int THREADS>
@@ -1473,7 +1603,12 @@ int fa_distill_loss(const fa_logits* x, const fa_teacher* t, float* loss, float*
     DistillArgs a = distill_args(x, t);
     a.loss = loss;
     a.stat = stat;
-    return launch_distill<true, false>(x, a, as_stream(stream));
+    switch (x->dtype) {
+        case FA_LOGITS_F32: launch_loss<FA_LOGITS_F32>(x, a, as_stream(stream)); break;
+        case FA_LOGITS_BF16: launch_loss<FA_LOGITS_BF16>(x, a, as_stream(stream)); break;
+        default: launch_loss<FA_LOGITS_F16>(x, a, as_stream(stream));
+    }
+    return hip_code(hipGetLastError());
 }
 
 int fa_distill_grad(const fa_logits* x, const fa_teacher* t, const float* stat, const float* row_grad, void* grad,
@@ -1489,7 +1624,12 @@ int fa_distill_grad(const fa_logits* x, const fa_teacher* t, const float* stat, 
     a.row_grad = row_grad;
     a.grad = grad;
     a.grad_rows = {x->inner, grad_stride_outer, grad_stride_inner};
-    return launch_distill<false, true>(x, a, as_stream(stream));
+    switch (x->dtype) {
+        case FA_LOGITS_F32: launch_grad<FA_LOGITS_F32>(x, a, as_stream(stream)); break;
+        case FA_LOGITS_BF16: launch_grad<FA_LOGITS_BF16>(x, a, as_stream(stream)); break;
+        default: launch_grad<FA_LOGITS_F16>(x, a, as_stream(stream));
+    }
+    return hip_code(hipGetLastError());
 }
 
 int fa_distill_loss_grad(const fa_logits* x, const fa_teacher* t, float* loss, void* grad, int64_t grad_stride_outer,
@@ -1505,7 +1645,12 @@ int fa_distill_loss_grad(const fa_logits* x, const fa_teacher* t, float* loss, v
     a.loss = loss;
     a.grad = grad;
     a.grad_rows = {x->inner, grad_stride_outer, grad_stride_inner};
-    return launch_distill<true, true>(x, a, as_stream(stream));
+    switch (x->dtype) {
+        case FA_LOGITS_F32: launch_step<FA_LOGITS_F32>(x, a, as_stream(stream)); break;
+        case FA_LOGITS_BF16: launch_step<FA_LOGITS_BF16>(x, a, as_stream(stream)); break;
+        default: launch_step<FA_LOGITS_F16>(x, a, as_stream(stream));
+    }
+    return hip_code(hipGetLastError());
 }
 
 int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int top, int32_t* out_ids,
