@@ -131,12 +131,11 @@ SIGNATURES = {
     "fa_half_buff_flush_mean": (_i, [_p, _p, _i, _sz, _i, _p]),
     "fa_half_fill": (_i, [_p, _d, _sz, _i, _p]),
     "fa_synth_fill": (_i, [_p, _p, _sz, _u64, _u64, _f, _p]),
-    "fa_token_workspace": (_i, [_p, _i, _p]),
-    "fa_token_scores": (_i, [_p, _p, C.c_int64, _i, _p, _p, _p, _p, _p, _p, _p]),
+    "fa_token_scores": (_i, [_p, _p, C.c_int64, _i, _p, _p, _p, _p, _p, _p]),
     "fa_merge_tops": (_i, [_p, _p, _i, C.c_int64, _i, _p, _p, _p]),
-    "fa_distill_loss": (_i, [_p, _p, _p, _p, _p, _p]),
+    "fa_distill_loss": (_i, [_p, _p, _p, _p, _p]),
     "fa_distill_grad": (_i, [_p, _p, _p, _p, _p, C.c_int64, C.c_int64, _p]),
-    "fa_distill_loss_grad": (_i, [_p, _p, _p, _p, C.c_int64, C.c_int64, _p, _p]),
+    "fa_distill_loss_grad": (_i, [_p, _p, _p, _p, C.c_int64, C.c_int64, _p]),
     "fa_pack_host": (_i, [_p, _p, _p, _p, _i, _i]),
     "fa_pack_host_window": (_i, [_p, _p, _p, _p, _i, _sz, _sz, _i]),
     "fa_host_copy_fresh": (_i, [_p, _p, _sz, _i]),
@@ -155,6 +154,8 @@ _lib: Optional[C.CDLL] = None
 def load() -> C.CDLL:
     """Load ``libappfl_amd.so`` once and attach the prototypes.  Raises if it is not built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -1566,23 +1566,14 @@ int launch_merge(const MergeArgs& a, int64_t rows, hipStream_t st) {
 
 extern "C" {
 
-int fa_token_workspace(const fa_logits* x, int top, size_t* bytes) {
-    const int rc = check_logits(x);
-    if (rc != FA_OK) return rc;
-    if (!bytes || top < 0 || top > FA_TOP_MAX) return FA_ERR_INVALID;
-    *bytes = 0;
-    return FA_OK;
-}
-
 int fa_token_scores(const fa_logits* x, const int64_t* targets, int64_t ignore_index, int top, float* logprob,
-                    float* entropy, float* lse, int32_t* top_ids, float* top_logprobs, void* ws, fa_stream_t stream) {
+                    float* entropy, float* lse, int32_t* top_ids, float* top_logprobs, fa_stream_t stream) {
     const int rc = check_logits(x);
     if (rc != FA_OK) return rc;
     if (top < 0 || top > FA_TOP_MAX || top > x->vocab) return FA_ERR_INVALID;
     const int64_t rows = x->outer * x->inner;
     if (rows == 0) return FA_OK;
     if (!entropy || !lse || (targets && !logprob) || (top && (!top_ids || !top_logprobs))) return FA_ERR_INVALID;
-    (void)ws;
     const ScoreArgs a = {x->data, rows_of(x), x->vocab, top, targets, ignore_index, logprob, entropy, lse,
                          top_logprobs, top_ids, scale_of(1.0)};
     switch (x->dtype) {
@@ -1593,13 +1584,12 @@ int fa_token_scores(const fa_logits* x, const int64_t* targets, int64_t ignore_i
     return hip_code(hipGetLastError());
 }
 
-int fa_distill_loss(const fa_logits* x, const fa_teacher* t, float* loss, float* stat, void* ws, fa_stream_t stream) {
+int fa_distill_loss(const fa_logits* x, const fa_teacher* t, float* loss, float* stat, fa_stream_t stream) {
     int rc = check_logits(x);
     if (rc == FA_OK) rc = check_teacher(t, x->outer * x->inner);
     if (rc != FA_OK) return rc;
     if (x->outer * x->inner == 0) return FA_OK;
     if (!loss || !stat) return FA_ERR_INVALID;
-    (void)ws;
     DistillArgs a = distill_args(x, t);
     a.loss = loss;
     a.stat = stat;
@@ -1633,14 +1623,13 @@ int fa_distill_grad(const fa_logits* x, const fa_teacher* t, const float* stat, 
 }
 
 int fa_distill_loss_grad(const fa_logits* x, const fa_teacher* t, float* loss, void* grad, int64_t grad_stride_outer,
-                         int64_t grad_stride_inner, void* ws, fa_stream_t stream) {
+                         int64_t grad_stride_inner, fa_stream_t stream) {
     int rc = check_logits(x);
     if (rc == FA_OK) rc = check_teacher(t, x->outer * x->inner);
     if (rc != FA_OK) return rc;
     if (x->outer * x->inner == 0) return FA_OK;
     if (!loss || !grad || grad_stride_outer < 0 || grad_stride_inner < 0) return FA_ERR_INVALID;
     if (!aligned_to(grad, elem_size(x->dtype))) return FA_ERR_ALIGN;
-    (void)ws;
     DistillArgs a = distill_args(x, t);
     a.loss = loss;
     a.grad = grad;

@@ -24,10 +24,14 @@ from typing import NamedTuple, Optional, Sequence, Tuple
 import torch
 
 from . import _native as N
-from .ops import _stream
 
 DTYPES = {torch.float32: N.FA_LOGITS_F32, torch.bfloat16: N.FA_LOGITS_BF16, torch.float16: N.FA_LOGITS_F16}
 TOP_MAX = N.FA_TOP_MAX
+
+# The smallest calls take less time on the GPU than in Python, so the checks below look at each
+# property once, and the stream's handle is read without making a Stream object.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_f32, _i32, _i64 = torch.float32, torch.int32, torch.int64
 
 
 class TokenScores(NamedTuple):
@@ -41,64 +45,62 @@ class TokenScores(NamedTuple):
 _here = contextlib.nullcontext()
 
 
-def _on(device: torch.device):
+def _on(index: int):
     """The tensors' device as the current one (launches go to the current device)."""
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _here if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
-def _on_device(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> None:
+def _check(name: str, t: torch.Tensor, dtype: torch.dtype, index: int, shape) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise N.NativeLibraryError(f"libappfl_amd kernels take device tensors; {name} is a CPU tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-
-
-def _shape(name: str, t: torch.Tensor, shape) -> None:
-    if tuple(t.shape) != tuple(shape):
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _logits(x: torch.Tensor) -> N.Logits:
-    _on_device("logits", x)
-    if x.dtype not in DTYPES:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"logits must be a tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise N.NativeLibraryError("libappfl_amd kernels take device tensors; logits is a CPU tensor")
+    code = DTYPES.get(x.dtype)
+    if code is None:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() == 2:
-        outer, inner, so, si = 1, x.shape[0], 0, x.stride(0)
-    elif x.dim() == 3:
-        outer, inner, so, si = x.shape[0], x.shape[1], x.stride(0), x.stride(1)
+    shape, stride = x.shape, x.stride()
+    if len(shape) == 2:
+        outer, inner, so, si = 1, shape[0], 0, stride[0]
+    elif len(shape) == 3:
+        outer, inner, so, si = shape[0], shape[1], stride[0], stride[1]
     else:
-        raise ValueError(f"logits must be [rows, vocab] or [batch, rows, vocab], got shape {tuple(x.shape)}")
-    vocab = x.shape[-1]
-    if vocab < 1 or vocab > N.FA_VOCAB_MAX:
+        raise ValueError(f"logits must be [rows, vocab] or [batch, rows, vocab], got shape {tuple(shape)}")
+    vocab = shape[-1]
+    if not 1 <= vocab <= N.FA_VOCAB_MAX:
         raise ValueError(f"a vocabulary of {vocab} tokens")
-    if x.stride(-1) != 1 and vocab > 1:
+    if stride[-1] != 1 and vocab > 1:
         raise ValueError("logits must have adjacent elements along the vocabulary")
     if outer * inner > 0x7FFFFFFF:
         raise ValueError("too many rows")
-    return N.Logits(x.data_ptr(), outer, inner, so, si, vocab, DTYPES[x.dtype])
+    return N.Logits(x.data_ptr(), outer, inner, so, si, vocab, code)
 
 
-def _list_pair(ids: torch.Tensor, logprobs: torch.Tensor, device: torch.device) -> None:
-    _on_device("ids", ids, device)
-    _on_device("logprobs", logprobs, device)
-    if ids.dtype != torch.int32:
-        raise TypeError(f"ids must be int32, got {ids.dtype}")
-    if logprobs.dtype != torch.float32:
-        raise TypeError(f"logprobs must be float32, got {logprobs.dtype}")
-    _shape("logprobs", logprobs, ids.shape)
-    k = ids.shape[-1]
+def _lists(ids: torch.Tensor, logprobs: torch.Tensor, index: int, lead) -> int:
+    """Checks a pair of lists for rows of shape `lead`; their length."""
+    if not isinstance(ids, torch.Tensor):
+        raise TypeError(f"ids must be a tensor, got {type(ids).__name__}")
+    shape = ids.shape
+    k = shape[-1] if len(shape) else 0
+    _check("ids", ids, _i32, index, lead + (k,))
+    _check("logprobs", logprobs, _f32, index, shape)
     if not 1 <= k <= TOP_MAX:
         raise ValueError(f"lists hold 1..{TOP_MAX} entries, got {k}")
     if k > 1 and (ids.stride(-1) != 1 or logprobs.stride(-1) != 1):
         raise ValueError("a list's entries must be adjacent")
-
-
-def _workspace(x: N.Logits, top: int, device: torch.device) -> Optional[torch.Tensor]:
-    need = C.c_size_t()
-    N.check(N.load().fa_token_workspace(C.byref(x), top, C.byref(need)), "fa_token_workspace")
-    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    return k
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -112,28 +114,26 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, t
     where it is `ignore_index`, NaN where it is outside the vocabulary) and the `top` most probable
     tokens, best first (ties to the lower id), with their log probabilities."""
     x = _logits(logits)
-    device = logits.device
-    if not isinstance(top, int) or isinstance(top, bool):
+    index = logits.get_device()
+    if type(top) is not int:
         raise TypeError("top must be an int")
     if not 0 <= top <= min(TOP_MAX, x.vocab):
         raise ValueError(f"top must be in 0..{min(TOP_MAX, x.vocab)}, got {top}")
     lead = logits.shape[:-1]
-    if targets is not None:
-        _on_device("targets", targets, device)
-        if targets.dtype != torch.int64:
-            raise TypeError(f"targets must be int64, got {targets.dtype}")
-        _shape("targets", targets, lead)
-        targets = targets.contiguous()
-    with _on(device):
-        entropy = torch.empty(lead, dtype=torch.float32, device=device)
-        lse = torch.empty(lead, dtype=torch.float32, device=device)
-        logprob = torch.empty(lead, dtype=torch.float32, device=device) if targets is not None else None
-        ids = torch.empty(lead + (top,), dtype=torch.int32, device=device) if top else None
-        tops = torch.empty(lead + (top,), dtype=torch.float32, device=device) if top else None
-        ws = _workspace(x, top, device)
-        rc = N.load().fa_token_scores(C.byref(x), _ptr(targets), int(ignore_index), top, _ptr(logprob),
-                                      entropy.data_ptr(), lse.data_ptr(), _ptr(ids), _ptr(tops), _ptr(ws),
-                                      _stream(logits))
+    logprob = ids = tops = None
+    with _on(index):
+        if targets is not None:
+            _check("targets", targets, _i64, index, lead)
+            targets = targets.contiguous()
+            logprob = logits.new_empty(lead, dtype=_f32)
+        entropy = logits.new_empty(lead, dtype=_f32)
+        lse = logits.new_empty(lead, dtype=_f32)
+        if top:
+            ids = logits.new_empty(lead + (top,), dtype=_i32)
+            tops = logits.new_empty(lead + (top,), dtype=_f32)
+        rc = N.load().fa_token_scores(C.byref(x), _ptr(targets), ignore_index, top, _ptr(logprob), entropy.data_ptr(),
+                                      lse.data_ptr(), _ptr(ids), _ptr(tops), _raw_stream(index))
+    if rc:
         N.check(rc, "fa_token_scores")
     return TokenScores(logprob, entropy, lse, ids, tops)
 
@@ -144,38 +144,36 @@ def merge_tops(ids: torch.Tensor, logprobs: torch.Tensor, weights: Sequence[floa
     weight per client (as in :func:`appfl_amd.ops.reduce_opt`), optionally a weight per client and
     row (``[K, rows]`` float32; nothing above zero leaves the client out of the row).  Returns ids
     and log probabilities ``[rows, top]``, best first; id -1 and -inf where a row has fewer tokens."""
-    _on_device("ids", ids)
+    if not isinstance(ids, torch.Tensor):
+        raise TypeError(f"ids must be a tensor, got {type(ids).__name__}")
     if ids.dim() != 3:
         raise ValueError(f"ids must be [clients, rows, k], got shape {tuple(ids.shape)}")
-    device = ids.device
-    _list_pair(ids, logprobs, device)
-    K, rows, k = ids.shape
+    index = ids.get_device()
+    K, rows, _ = ids.shape
+    k = _lists(ids, logprobs, index, ids.shape[:2])
     if len(weights) != K:
         raise ValueError("one weight per client")
-    w = [float(v) for v in weights]
     if not 1 <= K <= N.FA_MERGE_CLIENTS or K * k > N.FA_MERGE_ENTRIES:
         raise ValueError(f"one merge takes 1..{N.FA_MERGE_CLIENTS} clients and {N.FA_MERGE_ENTRIES} entries a row, "
                          f"got {K} clients of {k}")
-    if not all(v >= 0.0 and math.isfinite(v) for v in w):
+    w = N.double_array(weights)
+    if not all(0.0 <= v < math.inf for v in w):
         raise ValueError("client weights must be finite and not negative")
-    if not isinstance(top, int) or isinstance(top, bool):
+    if type(top) is not int:
         raise TypeError("top must be an int")
     if not 1 <= top <= min(K * k, TOP_MAX):
         raise ValueError(f"top must be in 1..{min(K * k, TOP_MAX)}, got {top}")
-    unit_client = unit_row = 0
+    unit, unit_stride = None, (0, 0)
     if token_weight is not None:
-        _on_device("token_weight", token_weight, device)
-        if token_weight.dtype != torch.float32:
-            raise TypeError(f"token_weight must be float32, got {token_weight.dtype}")
-        _shape("token_weight", token_weight, (K, rows))
-        unit_client, unit_row = token_weight.stride()
-    with _on(device):
-        out_ids = torch.empty((rows, top), dtype=torch.int32, device=device)
-        out_lp = torch.empty((rows, top), dtype=torch.float32, device=device)
-        tops = N.Tops(ids.data_ptr(), logprobs.data_ptr(), ids.stride(0), ids.stride(1), logprobs.stride(0),
-                      logprobs.stride(1), _ptr(token_weight), unit_client, unit_row, k)
-        rc = N.load().fa_merge_tops(C.byref(tops), N.double_array(w), K, rows, top, out_ids.data_ptr(),
-                                    out_lp.data_ptr(), _stream(ids))
+        _check("token_weight", token_weight, _f32, index, ids.shape[:2])
+        unit, unit_stride = token_weight.data_ptr(), token_weight.stride()
+    with _on(index):
+        out_ids = ids.new_empty((rows, top))
+        out_lp = logprobs.new_empty((rows, top))
+        tops = N.Tops(ids.data_ptr(), logprobs.data_ptr(), *ids.stride()[:2], *logprobs.stride()[:2], unit, *unit_stride, k)
+        rc = N.load().fa_merge_tops(C.byref(tops), w, K, rows, top, out_ids.data_ptr(), out_lp.data_ptr(),
+                                    _raw_stream(index))
+    if rc:
         N.check(rc, "fa_merge_tops")
     return out_ids, out_lp
 
@@ -184,20 +182,15 @@ def _teacher(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, te
              row_weight: Optional[torch.Tensor]):
     """The C structure and the tensors it points into (keep them until the call has returned)."""
     lead = logits.shape[:-1]
-    device = logits.device
-    _list_pair(ids, logprobs, device)
-    _shape("ids", ids, lead + ids.shape[-1:])
+    index = logits.get_device()
+    k = _lists(ids, logprobs, index, lead)
     tau = float(temperature)
     if not 1e-30 <= tau <= 1e30:
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     if row_weight is not None:
-        _on_device("row_weight", row_weight, device)
-        if row_weight.dtype != torch.float32:
-            raise TypeError(f"row_weight must be float32, got {row_weight.dtype}")
-        _shape("row_weight", row_weight, lead)
+        _check("row_weight", row_weight, _f32, index, lead)
         row_weight = row_weight.contiguous()
-    k = ids.shape[-1]
-    if ids.dim() == 3:                       # rows of a batch have to be one axis with one stride
+    if len(lead) == 2:                       # rows of a batch have to be one axis with one stride
         ids, logprobs = ids.reshape(-1, k), logprobs.reshape(-1, k)
     t = N.Teacher(ids.data_ptr(), logprobs.data_ptr(), ids.stride(0), logprobs.stride(0), _ptr(row_weight), tau, k)
     return t, (ids, logprobs, row_weight)
@@ -207,31 +200,35 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, temperature, row_weight):
         x = _logits(logits)
-        t, keep = _teacher(logits, ids, logprobs, temperature, row_weight)
-        device = logits.device
-        with _on(device):
-            loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-            stat = torch.empty(logits.shape[:-1] + (N.FA_DISTILL_STAT,), dtype=torch.float32, device=device)
-            ws = _workspace(x, 0, device)
-            N.check(N.load().fa_distill_loss(C.byref(x), C.byref(t), loss.data_ptr(), stat.data_ptr(), _ptr(ws),
-                                             _stream(logits)), "fa_distill_loss")
-        ctx.save_for_backward(logits, keep[0], keep[1], keep[2], stat)
+        index = logits.get_device()
+        with _on(index):
+            t, keep = _teacher(logits, ids, logprobs, temperature, row_weight)
+            lead = logits.shape[:-1]
+            loss = logits.new_empty(lead, dtype=_f32)
+            stat = logits.new_empty(lead + (N.FA_DISTILL_STAT,), dtype=_f32)
+            rc = N.load().fa_distill_loss(C.byref(x), C.byref(t), loss.data_ptr(), stat.data_ptr(), _raw_stream(index))
+        if rc:
+            N.check(rc, "fa_distill_loss")
+        ctx.save_for_backward(logits, stat, *keep)
         ctx.temperature = t.temperature
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, row_grad):
-        logits, ids, logprobs, row_weight, stat = ctx.saved_tensors
+        # pointers anew: hooks on saved tensors may hand back other memory than was saved
+        logits, stat, ids, logprobs, row_weight = ctx.saved_tensors
         x = _logits(logits)
         t = N.Teacher(ids.data_ptr(), logprobs.data_ptr(), ids.stride(0), logprobs.stride(0), _ptr(row_weight),
                       ctx.temperature, ids.shape[-1])
-        row_grad = row_grad.contiguous()
-        with _on(logits.device):
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            so, si = (0, grad.stride(0)) if grad.dim() == 2 else grad.stride()[:2]
-            N.check(N.load().fa_distill_grad(C.byref(x), C.byref(t), stat.data_ptr(), row_grad.data_ptr(),
-                                             grad.data_ptr(), so, si, _stream(logits)), "fa_distill_grad")
+        index = logits.get_device()
+        with _on(index):
+            row_grad = row_grad.contiguous()
+            grad = logits.new_empty(logits.shape)
+            rc = N.load().fa_distill_grad(C.byref(x), C.byref(t), stat.data_ptr(), row_grad.data_ptr(), grad.data_ptr(),
+                                          x.inner * x.vocab, x.vocab, _raw_stream(index))
+        if rc:
+            N.check(rc, "fa_distill_grad")
         return grad, None, None, None, None
 
 
@@ -252,19 +249,22 @@ def distill_loss_grad(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.T
     step of a caller that runs the model's backward from the logits' gradient.  `out` receives the
     gradient (the logits' shape and type; `logits` itself: written over them)."""
     x = _logits(logits)
-    t, keep = _teacher(logits, ids, logprobs, temperature, row_weight)
-    device = logits.device
-    with _on(device):
+    index = logits.get_device()
+    with _on(index):
+        t, keep = _teacher(logits, ids, logprobs, temperature, row_weight)
+        lead = logits.shape[:-1]
         if out is None:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+            out = logits.new_empty(logits.shape)
+            so, si = x.inner * x.vocab, x.vocab
         else:
             _check_out(out, logits)
             torch.autograd.graph.increment_version(out)      # a graph that saved it must not use it
-        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-        so, si = (0, out.stride(0)) if out.dim() == 2 else out.stride()[:2]
-        ws = _workspace(x, 0, device)
-        N.check(N.load().fa_distill_loss_grad(C.byref(x), C.byref(t), loss.data_ptr(), out.data_ptr(), so, si,
-                                              _ptr(ws), _stream(logits)), "fa_distill_loss_grad")
+            so, si = (0, out.stride(0)) if len(lead) == 1 else out.stride()[:2]
+        loss = logits.new_empty(lead, dtype=_f32)
+        rc = N.load().fa_distill_loss_grad(C.byref(x), C.byref(t), loss.data_ptr(), out.data_ptr(), so, si,
+                                           _raw_stream(index))
+    if rc:
+        N.check(rc, "fa_distill_loss_grad")
     return loss, out
 
 
@@ -275,10 +275,7 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
 
 
 def _check_out(out: torch.Tensor, logits: torch.Tensor) -> None:
-    _on_device("out", out, logits.device)
-    if out.dtype != logits.dtype:
-        raise TypeError(f"out must be {logits.dtype}, got {out.dtype}")
-    _shape("out", out, logits.shape)
+    _check("out", out, logits.dtype, logits.get_device(), logits.shape)
     if out.numel() == 0:
         return
     strides = sorted((s, n) for s, n in zip(out.stride(), out.shape) if n > 1)

@@ -528,11 +528,6 @@ typedef struct {             /* entry j of client c's row r at ids[c * id_client
     int k;                      /* 1..FA_TOP_MAX */
 } fa_tops;
 
-/* *bytes = size of the device workspace `ws` that the calls below need for these logits and `top`
- * (fa_token_scores; 0 for the distillation calls); 0: ws may be NULL.  Depends on the current
- * device's size.  A workspace belongs to one call at a time. */
-int fa_token_workspace(const fa_logits* logits, int top, size_t* bytes);
-
 /*
  * Per row:  lse = log sum_v exp x_v;  entropy = sum_v p_v (lse - x_v), p = exp(x - lse);
  *   logprob = x_target - lse (0 where target == ignore_index, NaN where it is outside the
@@ -543,7 +538,7 @@ int fa_token_workspace(const fa_logits* logits, int top, size_t* bytes);
  */
 int fa_token_scores(const fa_logits* logits, const int64_t* targets, int64_t ignore_index, int top,
                     float* logprob, float* entropy, float* lse, int32_t* top_ids,
-                    float* top_logprobs, void* ws, fa_stream_t stream);
+                    float* top_logprobs, fa_stream_t stream);
 
 /*
  * Weighted mean of K clients' answers, cut to its `top` largest entries:
@@ -572,13 +567,12 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
  * NaN.  A logit of -inf has q = 0 (loss inf where the teacher wants it).
  */
 int fa_distill_loss(const fa_logits* logits, const fa_teacher* teacher, float* loss, float* stat,
-                    void* ws, fa_stream_t stream);
+                    fa_stream_t stream);
 int fa_distill_grad(const fa_logits* logits, const fa_teacher* teacher, const float* stat,
                     const float* row_grad, void* grad, int64_t grad_stride_outer,
                     int64_t grad_stride_inner, fa_stream_t stream);
 int fa_distill_loss_grad(const fa_logits* logits, const fa_teacher* teacher, float* loss, void* grad,
-                         int64_t grad_stride_outer, int64_t grad_stride_inner, void* ws,
-                         fa_stream_t stream);
+                         int64_t grad_stride_outer, int64_t grad_stride_inner, fa_stream_t stream);
 
 /*
  * Host-side packing of one client's state dict into a row of a (pinned) staging slab:

@@ -41,12 +41,10 @@ INVALID, ALIGN, LARGE = -1, -2, -4
 def test_logits_are_checked_by_every_entry(change, code):
     lib = N.load()
     x, t = _logits(**change), _teacher()
-    need = C.c_size_t()
-    assert lib.fa_token_workspace(C.byref(x), 0, C.byref(need)) == code
-    assert lib.fa_token_scores(C.byref(x), None, 0, 0, None, 256, 256, None, None, None, None) == code
-    assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, 256, None, None) == code
+    assert lib.fa_token_scores(C.byref(x), None, 0, 0, None, 256, 256, None, None, None) == code
+    assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, 256, None) == code
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 256, 30, 10, None) == code
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None, None) == code
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None) == code
 
 
 @pytest.mark.parametrize("change", [
@@ -55,34 +53,30 @@ def test_logits_are_checked_by_every_entry(change, code):
 def test_teachers_are_checked(change):
     lib = N.load()
     x, t = _logits(), _teacher(**change)
-    assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, 256, None, None) == INVALID
+    assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, 256, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 256, 30, 10, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None) == INVALID
 
 
 def test_outputs_and_null_pointers_are_checked():
     lib = N.load()
-    x, t, need = _logits(), _teacher(), C.c_size_t()
-    assert lib.fa_token_workspace(None, 0, C.byref(need)) == INVALID
-    assert lib.fa_token_workspace(C.byref(x), 0, None) == INVALID
-    assert lib.fa_token_workspace(C.byref(x), -1, C.byref(need)) == INVALID
-    assert lib.fa_token_workspace(C.byref(x), 257, C.byref(need)) == INVALID
+    x, t = _logits(), _teacher()
     scores = lambda **c: lib.fa_token_scores(C.byref(x), *{**dict(
-        targets=None, ignore=0, top=0, logprob=None, entropy=256, lse=256, ids=None, lps=None, ws=None, st=None), **c}.values())
+        targets=None, ignore=0, top=0, logprob=None, entropy=256, lse=256, ids=None, lps=None, st=None), **c}.values())
     for change in (dict(entropy=None), dict(lse=None), dict(targets=256), dict(top=2), dict(top=2, ids=256), dict(top=11),
                    dict(top=-1)):
         assert scores(**change) == INVALID, change
-    assert lib.fa_distill_loss(C.byref(x), None, 256, 256, None, None) == INVALID
-    assert lib.fa_distill_loss(C.byref(x), C.byref(t), None, 256, None, None) == INVALID
-    assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, None, None, None) == INVALID
+    assert lib.fa_distill_loss(C.byref(x), None, 256, 256, None) == INVALID
+    assert lib.fa_distill_loss(C.byref(x), C.byref(t), None, 256, None) == INVALID
+    assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, None, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), None, None, 256, 30, 10, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, None, 30, 10, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 256, -1, 10, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 258, 30, 10, None) == ALIGN
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, None, 30, 10, None, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, 256, 30, 10, None, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, -10, None, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 257, 30, 10, None, None) == ALIGN
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, None, 30, 10, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, 256, 30, 10, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, -10, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 257, 30, 10, None) == ALIGN
 
 
 def test_merge_arguments_are_checked():
@@ -106,10 +100,10 @@ def test_merge_arguments_are_checked():
 def test_empty_calls_do_nothing():
     lib = N.load()
     x, t = _logits(outer=0, data=None), _teacher()
-    assert lib.fa_token_scores(C.byref(x), None, 0, 0, None, None, None, None, None, None, None) == 0
-    assert lib.fa_distill_loss(C.byref(x), C.byref(t), None, None, None, None) == 0
+    assert lib.fa_token_scores(C.byref(x), None, 0, 0, None, None, None, None, None, None) == 0
+    assert lib.fa_distill_loss(C.byref(x), C.byref(t), None, None, None) == 0
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), None, None, None, 0, 0, None) == 0
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, None, 0, 0, None, None) == 0
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, None, 0, 0, None) == 0
     tops = _tops()
     assert lib.fa_merge_tops(C.byref(tops), N.double_array([1.0]), 1, 0, 4, None, None, None) == 0
 
