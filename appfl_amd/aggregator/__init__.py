@@ -5,6 +5,7 @@ from .base_aggregator import BaseAggregator
 from .fedavg_aggregator import (FedAdagradAggregator, FedAdamAggregator, FedAvgAggregator,
                                 FedAvgMAggregator, FedYogiAggregator)
 from .fedasync_aggregator import FedAsyncAggregator, FedBuffAggregator
+from .feddistill_aggregator import FedDistillAggregator
 from .fedcompass_aggregator import FedCompassAggregator, FedQueueAggregator
 
 __all__ = [
@@ -20,4 +21,5 @@ __all__ = [
     "FedQueueAggregator",
     "IIADMMAggregator",
     "ICEADMMAggregator",
+    "FedDistillAggregator",
 ]

@@ -104,6 +104,20 @@ def register_staging_scheduler(prefix: str = "MI355X", replace: bool = False, mo
     return out
 
 
+def register_distillation(module=None) -> Dict[str, type]:
+    """Install `FedDistillAggregator`, which has no stock counterpart, into
+    `appfl.algorithm.aggregator` (or `module`) under its own name, as a subclass of that module's
+    `BaseAggregator` if it has one, so that `aggregator: "FedDistillAggregator"` in a server YAML
+    resolves to it."""
+    target = module if module is not None else importlib.import_module("appfl.algorithm.aggregator")
+    ours = _dev.FedDistillAggregator
+    base = getattr(target, "BaseAggregator", None)
+    bases = (ours,) if base is None or issubclass(ours, base) else (ours, base)
+    cls = type("FedDistillAggregator", bases, {"__module__": ours.__module__, "__doc__": ours.__doc__})
+    setattr(target, "FedDistillAggregator", cls)
+    return {"FedDistillAggregator": cls}
+
+
 def register(prefix: str = "MI355X", replace: bool = False, module=None,
              stage_on_arrival: bool = False, scheduler_module=None) -> Dict[str, type]:
     """Install the device aggregators into `appfl.algorithm.aggregator` (or `module`) and, with
