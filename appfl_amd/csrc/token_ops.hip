@@ -1193,9 +1193,9 @@ __global__ __launch_bounds__(THREADS) void distill_step_kernel(const DistillArgs
 // group's largest below 2^51: at most 2^13 entries stay below 2^64, whole numbers add up to the same
 // sum in any order, and a sum is off by no more than 2^-51 of the largest term per entry (fp64
 // additions: 2^-53 of the sum each).  The groups' values are then ranked, ties to the lowest id.
-// A table takes kFull<THREADS> different tokens; a row with more is merged in rounds, each of which
-// takes the tokens that got into the table and ranks them together with the best of the rounds
-// before.
+// A table takes kFull different tokens, and those that are on their way when it fills; a row with more
+// is merged in rounds, each of which takes the tokens that got into the table and ranks them together
+// with the best of the rounds before.
 struct MergeArgs {
     const int32_t* ids;
     const float* lp;
@@ -1209,140 +1209,196 @@ struct MergeArgs {
     double w[FA_MERGE_CLIENTS];
 };
 
-struct Ranked {
-    uint64_t key;                // the value's bits; a NaN's are the largest
-    unsigned id;
-};
-
 __device__ __forceinline__ bool before(uint64_t ka, unsigned ia, uint64_t kb, unsigned ib) {
     return ka > kb || (ka == kb && ia < ib);
 }
 
-template <int THREADS>
-struct MergeLds {
-    static constexpr int kSlots = 4 * THREADS;
-    static constexpr int kFull = 3 * THREADS;      // tokens after which none is added; THREADS more may be under way
-    double share[FA_MERGE_CLIENTS];
-    unsigned answered[FA_MERGE_CLIENTS / 32];
-    unsigned token[kSlots];                        // id, ~0: free
-    unsigned peak[kSlots];                         // exponent of the group's largest term
-    uint64_t sum[kSlots];
-    uint64_t key[kSlots + FA_TOP_MAX];             // by group, in the order of their coming, then the list so far
-    unsigned id[kSlots + FA_TOP_MAX];
-    u16 slot[kSlots];                              // by group
-    uint64_t bound[THREADS];
-    unsigned bound_id[THREADS];
-    unsigned count, open, kept;
-    uint64_t limit;
-    unsigned limit_id;
-    double total;
-};
-
 constexpr unsigned kFree = ~0u;
 constexpr unsigned kExpInf = 2047;
 
-template <int THREADS>
-__device__ __forceinline__ int find_slot(const MergeLds<THREADS>& l, unsigned id, unsigned& at) {
-    // the slot of `id` (>= 0), or -1 with `at` the free slot met first, or at = kFree in a full table
-    constexpr unsigned kMask = MergeLds<THREADS>::kSlots - 1;
-    for (unsigned n = 0; n <= kMask; ++n) {
+// ROUNDS: rows may hold more different tokens than the table takes.
+template <int SLOTS, bool ROUNDS>
+struct MergeLds {
+    static constexpr int kFull = SLOTS * 3 / 4;
+    static constexpr int kList = ROUNDS ? FA_TOP_MAX : 0;
+    static constexpr int kAll = SLOTS + kList + 8;
+    static constexpr int kBest = SLOTS < FA_TOP_MAX ? SLOTS : FA_TOP_MAX;
+    double share[FA_MERGE_CLIENTS];
+    unsigned answered[FA_MERGE_CLIENTS];
+    unsigned token[kAll];                          // by slot: id, ~0: free.  Later by group: id
+    uint64_t sum[kAll];                            // by slot: sum.  Later by group: the value's bits
+    unsigned peak[SLOTS];                          // exponent of the group's largest term
+    u16 slot[SLOTS];                               // by group, in the order of their coming
+    uint64_t list_key[kList + 1];                  // the best of the rounds before
+    unsigned list_id[kList + 1];
+    uint64_t best[kBest];                          // the ranked values
+    unsigned count, open, left, bound;
+    double total;
+};
+
+// The slot of `id` (< 2^31), or -1 with `at` the free slot met first, kFree in a full table.
+template <int SLOTS, bool ROUNDS>
+__device__ __forceinline__ int find_slot(const MergeLds<SLOTS, ROUNDS>& l, unsigned id, unsigned& at) {
+    for (int n = 0; n < SLOTS; ++n) {
         const unsigned t = __hip_atomic_load(&l.token[at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         if (t == id) return static_cast<int>(at);
         if (t == kFree) return -1;
-        at = (at + 1) & kMask;
+        at = (at + 1) & (SLOTS - 1);
     }
     at = kFree;
     return -1;
 }
 
-template <int THREADS>
+template <int SLOTS>
 __device__ __forceinline__ unsigned hash_of(unsigned id) {
-    constexpr int kBits = __builtin_ctz(MergeLds<THREADS>::kSlots);
-    return (id * 0x9e3779b1u) >> (32 - kBits);
+    return (id * 0x9e3779b1u) >> (32 - __builtin_ctz(SLOTS));
+}
+
+// The slot of `id`, put into the table if need be; -1: no room.
+template <int SLOTS, bool ROUNDS>
+__device__ __forceinline__ int take_slot(MergeLds<SLOTS, ROUNDS>& l, unsigned id, unsigned at) {
+    for (;;) {
+        const int s = find_slot(l, id, at);
+        if (s >= 0) return s;
+        if (at == kFree) return -1;
+        if (ROUNDS && __hip_atomic_load(&l.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) >=
+                          MergeLds<SLOTS, ROUNDS>::kFull)
+            return -1;
+        if (atomicCAS(&l.token[at], kFree, id) == kFree) {
+            l.slot[atomicAdd(&l.count, 1u)] = static_cast<u16>(at);
+            return static_cast<int>(at);
+        }                                          // taken meanwhile, perhaps by this very token: look again
+    }
+}
+
+__device__ __forceinline__ unsigned exponent_of(double p) { return static_cast<unsigned>(__double2hiint(p)) >> 20 & 2047u; }
+
+// Waves a SIMD holds, so that the compiler keeps to their registers: as many as LDS lets in.
+constexpr int merge_waves(int threads, int per) { return per >= 8 ? 4 : threads == 64 ? 3 : 6; }
+
+// e^v of an fp32 value in fp64: 2^n times the Taylor series of e^r, |r| <= ln 2 / 2, whose first
+// omitted term is below 2^-57; log2(e) in two parts keeps r exact to fp64.  About half the
+// instructions of the library's, which has to take any fp64 argument.
+__device__ __forceinline__ double exp_of(float v) {
+    const double x = static_cast<double>(fminf(fmaxf(v, -1000.0f), 1000.0f));       // beyond: 0 and inf; NaN see below
+    const double n = rint(x * 1.4426950408889634);
+    const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));   // ln 2 in two parts
+    double e = 1.0 / 6227020800.0;                                                  // 1 / 13!
+    e = fma(e, r, 1.0 / 479001600.0);
+    e = fma(e, r, 1.0 / 39916800.0);
+    e = fma(e, r, 1.0 / 3628800.0);
+    e = fma(e, r, 1.0 / 362880.0);
+    e = fma(e, r, 1.0 / 40320.0);
+    e = fma(e, r, 1.0 / 5040.0);
+    e = fma(e, r, 1.0 / 720.0);
+    e = fma(e, r, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    return v != v ? __builtin_nan("") : ldexp(e, static_cast<int>(n));
 }
 
 // PER entries per thread
-template <int THREADS, int PER>
-__global__ __launch_bounds__(THREADS, PER <= 16 ? 4 : 2) void merge_tops_kernel(const MergeArgs a) {
-    using L = MergeLds<THREADS>;
+template <int THREADS, int PER, int SLOTS, bool ROUNDS>
+__global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops_kernel(const MergeArgs a) {
+    using L = MergeLds<SLOTS, ROUNDS>;
+    constexpr int kGroupsPer = (SLOTS + THREADS - 1) / THREADS;
     __shared__ L l;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x;
     const int n = a.K * a.k;
-    for (int c = tid; c < a.K; c += THREADS)
+    // entry e of a thread is i = tid + e * THREADS = (client, place) = (i / k, i % k)
+    const int c0 = static_cast<int>((static_cast<uint64_t>(tid) * a.per_k) >> 32);
+    const int dc = static_cast<int>((static_cast<uint64_t>(THREADS) * a.per_k) >> 32), dj = THREADS - dc * a.k;
+    unsigned id[PER];
+    float lp[PER];
+    {
+        int j = tid - c0 * a.k;
+        const int32_t* ip = a.ids + row * a.id_row + c0 * a.id_client + j;
+        const float* lpp = a.lp + row * a.lp_row + c0 * a.lp_client + j;
+        const int64_t id_step = dc * a.id_client + dj, id_wrap = a.id_client - a.k;
+        const int64_t lp_step = dc * a.lp_client + dj, lp_wrap = a.lp_client - a.k;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const bool in = tid + e * THREADS < n;
+            id[e] = in ? static_cast<unsigned>(*ip) : kFree;
+            lp[e] = in ? *lpp : 0.0f;
+            j += dj;
+            const bool wrap = j >= a.k;
+            j -= wrap ? a.k : 0;
+            ip += id_step + (wrap ? id_wrap : 0);
+            lpp += lp_step + (wrap ? lp_wrap : 0);
+        }
+    }
+    for (int c = tid; c < a.K; c += THREADS) {
         l.share[c] = a.w[c] * static_cast<double>(a.unit ? a.unit[c * a.unit_client + row * a.unit_row] : 1.0f);
-    if (tid < FA_MERGE_CLIENTS / 32) l.answered[tid] = 0;
-    for (int i = tid; i < L::kSlots; i += THREADS) {
+        l.answered[c] = 0;
+    }
+    for (int i = tid; i < SLOTS; i += THREADS) {
         l.token[i] = kFree;
         l.peak[i] = 0;
         l.sum[i] = 0;
     }
-    if (tid == 0) l.count = l.open = l.kept = 0;
-    __syncthreads();
+    if (tid == 0) l.count = l.open = 0;
 
-    unsigned id[PER];
+    __syncthreads();
     double p[PER];
     int slot[PER];                                 // -1: waiting, -2: absent or done
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        const int i = tid + e * THREADS;
-        slot[e] = -2;
-        id[e] = 0;
-        p[e] = 0.0;
-        if (i < n) {
-            const int c = static_cast<int>((static_cast<uint64_t>(i) * a.per_k) >> 32), j = i - c * a.k;
-            const int v = a.ids[c * a.id_client + row * a.id_row + j];
-            const float lp = a.lp[c * a.lp_client + row * a.lp_row + j];
-            const double share = l.share[c];
-            if (v >= 0 && share > 0.0) {
-                id[e] = static_cast<unsigned>(v);
-                p[e] = share * exp(static_cast<double>(lp));
-                slot[e] = -1;
-                atomicOr(&l.answered[c / 32], 1u << (c % 32));
-            }
-        }
-    }
-    int have = 0;
-    for (bool more = true; more;) {
-        // tokens into the table
-        bool waiting = false;
+    {
+        int c = c0, j = tid - c0 * a.k;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            if (slot[e] != -1) continue;
-            unsigned at = hash_of<THREADS>(id[e]);
-            for (;;) {
-                const int s = find_slot(l, id[e], at);
-                if (s >= 0) {
-                    slot[e] = s;
-                    break;
+            slot[e] = -2;
+            p[e] = 0.0;
+            if (static_cast<int>(id[e]) >= 0) {    // entries past the end are absent
+                const double share = l.share[c];
+                if (share > 0.0) {
+                    p[e] = share * exp_of(lp[e]);
+                    slot[e] = -1;
+                    l.answered[c] = 1;
                 }
-                if (at == kFree || __hip_atomic_load(&l.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) >= L::kFull) break;
-                const unsigned old = atomicCAS(&l.token[at], kFree, id[e]);
-                if (old == kFree) {
-                    l.slot[atomicAdd(&l.count, 1u)] = static_cast<u16>(at);
-                    slot[e] = static_cast<int>(at);
-                    break;
-                }                                  // taken meanwhile, perhaps by this very token: look again
             }
-            if (slot[e] >= 0)
-                atomicMax(&l.peak[slot[e]], static_cast<unsigned>(__double2hiint(p[e])) >> 20 & 2047u);
-            else
-                waiting = true;
+            j += dj;
+            const bool wrap = j >= a.k;
+            j -= wrap ? a.k : 0;
+            c += dc + (wrap ? 1 : 0);
         }
-        if (waiting) l.open = 1;
+    }
+    int kept = 0;
+    for (bool more = true; more;) {
+        // tokens into the table: the first entries bring most of them, the others mostly find theirs
+        // at the first look, and those looks are on their way together
+        bool waiting = false;
+        if (slot[0] == -1) slot[0] = take_slot(l, id[0], hash_of<SLOTS>(id[0]));
+        unsigned seen[PER];
+#pragma unroll
+        for (int e = 1; e < PER; ++e)
+            seen[e] = __hip_atomic_load(&l.token[hash_of<SLOTS>(id[e])], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            if (e && slot[e] == -1) {
+                const unsigned at = hash_of<SLOTS>(id[e]);
+                slot[e] = seen[e] == id[e] ? static_cast<int>(at) : take_slot(l, id[e], at);
+            }
+            if (slot[e] >= 0) atomicMax(&l.peak[slot[e]], exponent_of(p[e]));
+            waiting = waiting || slot[e] == -1;
+        }
+        if (ROUNDS && waiting) l.open = 1;
         __syncthreads();
-        more = l.open != 0;
+        more = ROUNDS && l.open != 0;
         const int groups = static_cast<int>(l.count);
         if (more) {
             // entries that found no room: their token may have come in through another entry
 #pragma unroll
             for (int e = 0; e < PER; ++e) {
                 if (slot[e] != -1) continue;
-                unsigned at = hash_of<THREADS>(id[e]);
+                unsigned at = hash_of<SLOTS>(id[e]);
                 const int s = find_slot(l, id[e], at);
                 if (s < 0) continue;
                 slot[e] = s;
-                atomicMax(&l.peak[s], static_cast<unsigned>(__double2hiint(p[e])) >> 20 & 2047u);
+                atomicMax(&l.peak[s], exponent_of(p[e]));
             }
             __syncthreads();
         }
@@ -1362,68 +1418,142 @@ __global__ __launch_bounds__(THREADS, PER <= 16 ? 4 : 2) void merge_tops_kernel(
             slot[e] = -2;
         }
         __syncthreads();
-        // the groups' values, behind them the list so far
-        for (int g = tid; g < groups; g += THREADS) {
-            const int s = l.slot[g];
-            const unsigned x = l.peak[s];
-            const uint64_t sum = l.sum[s];
-            double v;
-            if (x == kExpInf)
-                v = sum >> 32 ? __builtin_nan("") : __builtin_inf();
-            else
-                v = ldexp(static_cast<double>(sum), static_cast<int>(x ? x : 1) - 1022 - 51);
-            l.key[g] = v != v ? 0x7ff8000000000000ull : static_cast<uint64_t>(__double_as_longlong(v));
-            l.id[g] = l.token[s];
-            l.token[s] = kFree;
-            l.peak[s] = 0;
-            l.sum[s] = 0;
-        }
-        const int kept = static_cast<int>(l.kept);
-        for (int j = tid; j < kept; j += THREADS) {
-            l.key[groups + j] = l.bound[j];
-            l.id[groups + j] = l.bound_id[j];
+        // the groups' values, moved together; behind them the list so far
+        uint64_t key[kGroupsPer];
+        unsigned name[kGroupsPer];
+#pragma unroll
+        for (int e = 0; e < kGroupsPer; ++e) {
+            const int g = tid + e * THREADS;
+            key[e] = 0;
+            name[e] = kFree;
+            if (g < groups) {
+                const int s = l.slot[g];
+                const unsigned x = l.peak[s];
+                const uint64_t sum = l.sum[s];
+                name[e] = l.token[s];
+                const double v = x == kExpInf ? (sum >> 32 ? __builtin_nan("") : __builtin_inf())
+                                              : ldexp(static_cast<double>(sum), static_cast<int>(x ? x : 1) - 1022 - 51);
+                key[e] = v != v ? 0x7ff8000000000000ull : static_cast<uint64_t>(__double_as_longlong(v));
+            }
         }
         __syncthreads();
-        const int total = groups + kept;
-        have = total < a.top ? total : a.top;
-        // ranks
-        for (int g = tid; g < total; g += THREADS) {
-            const uint64_t key = l.key[g];
-            const unsigned me = l.id[g];
-            int rank = 0;
-            for (int o = 0; o < total; ++o) rank += before(l.key[o], l.id[o], key, me);
-            if (rank < a.top) {
-                if (more) {
-                    l.bound[rank] = key;
-                    l.bound_id[rank] = me;
-                } else {
-                    a.out_ids[row * a.top + rank] = static_cast<int32_t>(me);
-                    l.bound[rank] = key;
+        // of many, only what reaches a bound that `top` of the threads' best reach
+        unsigned least = 0;
+        if (groups > 96 && groups >= 2 * a.top && a.top < THREADS / 2) {
+            unsigned best = 0;
+#pragma unroll
+            for (int e = 0; e < kGroupsPer; ++e) {
+                const unsigned hi = name[e] != kFree ? static_cast<unsigned>(key[e] >> 32) + 1 : 0;
+                best = hi > best ? hi : best;
+            }
+            l.peak[tid] = best;
+            __syncthreads();
+            if (tid < kWave) {
+                unsigned v[THREADS / kWave];
+#pragma unroll
+                for (int i = 0; i < THREADS / kWave; ++i) v[i] = l.peak[i * kWave + tid];
+                int reach;
+                const unsigned nth = wave_nth(v, a.top, reach);
+                if (tid == 0) l.bound = nth;
+            }
+            if (tid == 0) l.left = 0;
+            __syncthreads();
+            least = l.bound;
+        }
+        int total = groups;
+        if (least) {
+#pragma unroll
+            for (int e = 0; e < kGroupsPer; ++e) {
+                const bool in = name[e] != kFree && static_cast<unsigned>(key[e] >> 32) + 1 >= least;
+                const uint64_t m = __ballot(in);
+                unsigned base = 0;
+                if (m && tid % kWave == 0) base = atomicAdd(&l.left, static_cast<unsigned>(__popcll(m)));
+                base = __builtin_amdgcn_readfirstlane(base);
+                if (in) {
+                    l.sum[base + lanes_below(m)] = key[e];
+                    l.token[base + lanes_below(m)] = name[e];
+                }
+            }
+            __syncthreads();
+            total = static_cast<int>(l.left);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kGroupsPer; ++e) {
+                const int g = tid + e * THREADS;
+                if (g < groups) {
+                    l.sum[g] = key[e];
+                    l.token[g] = name[e];
                 }
             }
         }
-        if (tid == 0) {
-            l.count = l.open = 0;
-            l.kept = have;
+        if (ROUNDS)
+            for (int j = tid; j < kept; j += THREADS) {
+                l.sum[total + j] = l.list_key[j];
+                l.token[total + j] = l.list_id[j];
+            }
+        total += kept;
+        if (tid < 8) {                             // ranks below everything
+            l.sum[total + tid] = 0;
+            l.token[total + tid] = kFree;
         }
         __syncthreads();
+        kept = total < a.top ? total : a.top;
+        // ranks: `share` neighbouring threads count for one value
+        int share = 1;
+        while (share < 16 && total * share * 2 <= THREADS) share *= 2;
+        for (int g0 = 0; g0 < total; g0 += THREADS / share) {
+            const int g = g0 + tid / share, part = tid % share;
+            const uint64_t mine = l.sum[g < total ? g : total];
+            const unsigned me = l.token[g < total ? g : total];
+            int rank = 0;
+            for (int o = part * 8; o < total; o += share * 8) {
+                uint64_t k8[8];
+                unsigned i8[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    k8[q] = l.sum[o + q];
+                    i8[q] = l.token[o + q];
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) rank += before(k8[q], i8[q], mine, me);
+            }
+            for (int d = 1; d < share; d *= 2) rank += __shfl_xor(rank, d);
+            if (part || g >= total || rank >= a.top) continue;
+            if (more) {
+                l.list_key[rank] = mine;
+                l.list_id[rank] = me;
+            } else {
+                a.out_ids[row * a.top + rank] = static_cast<int32_t>(me);
+                l.best[rank] = mine;
+            }
+        }
+        if (more) {
+            __syncthreads();
+            for (int i = tid; i < SLOTS; i += THREADS) {
+                l.token[i] = kFree;
+                l.peak[i] = 0;
+                l.sum[i] = 0;
+            }
+            if (tid == 0) l.count = l.open = 0;
+            __syncthreads();
+        }
     }
     if (tid < kWave) {
         double t = 0.0;
         for (int c = tid; c < a.K; c += kWave)
-            if (l.answered[c / 32] >> (c % 32) & 1) t += l.share[c];
+            if (l.answered[c]) t += l.share[c];
         for (int d = kWave / 2; d > 0; d >>= 1) t += __shfl_xor(t, d);
         if (tid == 0) l.total = t;
     }
     __syncthreads();
     const double total = l.total;
     for (int j = tid; j < a.top; j += THREADS) {
-        float lp = -kInf;
-        if (j < have)
-            lp = static_cast<float>(log(__longlong_as_double(static_cast<long long>(l.bound[j])) / total));
+        float out = -kInf;
+        if (j < kept)
+            out = static_cast<float>(log(__longlong_as_double(static_cast<long long>(l.best[j])) / total));
         else
             a.out_ids[row * a.top + j] = -1;
-        a.out_lp[row * a.top + j] = lp;
+        a.out_lp[row * a.top + j] = out;
     }
 }
 
@@ -1546,19 +1676,22 @@ void launch_scores(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
 
 hipStream_t as_stream(fa_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
-template <int THREADS, int PER>
+template <int THREADS, int PER, int SLOTS, bool ROUNDS>
 void launch_merge_t(const MergeArgs& a, int64_t rows, hipStream_t st) {
-    hipLaunchKernelGGL((merge_tops_kernel<THREADS, PER>), dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((merge_tops_kernel<THREADS, PER, SLOTS, ROUNDS>), dim3(static_cast<unsigned>(rows)), dim3(THREADS),
+                       0, st, a);
 }
 
+// Threads for at most 16 entries each; a table that holds every token of a short list at once.
 int launch_merge(const MergeArgs& a, int64_t rows, hipStream_t st) {
     const int n = a.K * a.k;
-    if (n <= 256) launch_merge_t<256, 1>(a, rows, st);
-    else if (n <= 512) launch_merge_t<256, 2>(a, rows, st);
-    else if (n <= 1024) launch_merge_t<256, 4>(a, rows, st);
-    else if (n <= 2048) launch_merge_t<256, 8>(a, rows, st);
-    else if (n <= 4096) launch_merge_t<256, 16>(a, rows, st);
-    else launch_merge_t<256, 32>(a, rows, st);
+    if (n <= 64) launch_merge_t<64, 1, 128, false>(a, rows, st);
+    else if (n <= 256) launch_merge_t<64, 4, 512, false>(a, rows, st);
+    else if (n <= 512) launch_merge_t<256, 2, 1024, false>(a, rows, st);
+    else if (n <= 1024) launch_merge_t<256, 4, 1024, true>(a, rows, st);
+    else if (n <= 2048) launch_merge_t<512, 4, 1024, true>(a, rows, st);
+    else if (n <= 4096) launch_merge_t<512, 8, 1024, true>(a, rows, st);
+    else launch_merge_t<512, 16, 1024, true>(a, rows, st);
     return hip_code(hipGetLastError());
 }
 
