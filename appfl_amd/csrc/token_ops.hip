@@ -1274,7 +1274,7 @@ __device__ __forceinline__ int take_slot(MergeLds<SLOTS, ROUNDS>& l, unsigned id
 __device__ __forceinline__ unsigned exponent_of(double p) { return static_cast<unsigned>(__double2hiint(p)) >> 20 & 2047u; }
 
 // Waves a SIMD holds, so that the compiler keeps to their registers: as many as LDS lets in.
-constexpr int merge_waves(int threads, int per) { return per >= 8 ? 4 : threads == 64 ? 3 : 6; }
+constexpr int merge_waves(int threads, int per) { return per >= 8 ? 4 : threads == 256 && per == 4 ? 5 : 6; }
 
 // e^v of an fp32 value in fp64: 2^n times the Taylor series of e^r, |r| <= ln 2 / 2, whose first
 // omitted term is below 2^-57; log2(e) in two parts keeps r exact to fp64.  About half the
@@ -1344,22 +1344,19 @@ __global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops
     if (tid == 0) l.count = l.open = 0;
 
     __syncthreads();
+    // at[e]: the entry's id while it waits for a slot, kSlot + its slot, kFree: absent or done
+    constexpr unsigned kSlot = 1u << 31;
+    unsigned (&at)[PER] = id;
     double p[PER];
-    int slot[PER];                                 // -1: waiting, -2: absent or done
     {
         int c = c0, j = tid - c0 * a.k;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            slot[e] = -2;
-            p[e] = 0.0;
-            if (static_cast<int>(id[e]) >= 0) {    // entries past the end are absent
-                const double share = l.share[c];
-                if (share > 0.0) {
-                    p[e] = share * exp_of(lp[e]);
-                    slot[e] = -1;
-                    l.answered[c] = 1;
-                }
-            }
+            double share = 0.0;
+            if (static_cast<int>(at[e]) >= 0) share = l.share[c];      // entries past the end are absent
+            p[e] = share * exp_of(lp[e]);
+            if (share > 0.0) l.answered[c] = 1;
+            else at[e] = kFree;
             j += dj;
             const bool wrap = j >= a.k;
             j -= wrap ? a.k : 0;
@@ -1371,19 +1368,23 @@ __global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops
         // tokens into the table: the first entries bring most of them, the others mostly find theirs
         // at the first look, and those looks are on their way together
         bool waiting = false;
-        if (slot[0] == -1) slot[0] = take_slot(l, id[0], hash_of<SLOTS>(id[0]));
         unsigned seen[PER];
 #pragma unroll
-        for (int e = 1; e < PER; ++e)
-            seen[e] = __hip_atomic_load(&l.token[hash_of<SLOTS>(id[e])], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-#pragma unroll
         for (int e = 0; e < PER; ++e) {
-            if (e && slot[e] == -1) {
-                const unsigned at = hash_of<SLOTS>(id[e]);
-                slot[e] = seen[e] == id[e] ? static_cast<int>(at) : take_slot(l, id[e], at);
+            if (e == 1) {
+#pragma unroll
+                for (int o = 1; o < PER; ++o)
+                    seen[o] = __hip_atomic_load(&l.token[hash_of<SLOTS>(at[o])], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
-            if (slot[e] >= 0) atomicMax(&l.peak[slot[e]], exponent_of(p[e]));
-            waiting = waiting || slot[e] == -1;
+            if (static_cast<int>(at[e]) < 0) continue;
+            const unsigned first = hash_of<SLOTS>(at[e]);
+            const int s = e && seen[e] == at[e] ? static_cast<int>(first) : take_slot(l, at[e], first);
+            if (s >= 0) {
+                at[e] = kSlot + s;
+                atomicMax(&l.peak[s], exponent_of(p[e]));
+            } else {
+                waiting = true;
+            }
         }
         if (ROUNDS && waiting) l.open = 1;
         __syncthreads();
@@ -1393,19 +1394,19 @@ __global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops
             // entries that found no room: their token may have come in through another entry
 #pragma unroll
             for (int e = 0; e < PER; ++e) {
-                if (slot[e] != -1) continue;
-                unsigned at = hash_of<SLOTS>(id[e]);
-                const int s = find_slot(l, id[e], at);
+                if (static_cast<int>(at[e]) < 0) continue;
+                unsigned look = hash_of<SLOTS>(at[e]);
+                const int s = find_slot(l, at[e], look);
                 if (s < 0) continue;
-                slot[e] = s;
+                at[e] = kSlot + s;
                 atomicMax(&l.peak[s], exponent_of(p[e]));
             }
             __syncthreads();
         }
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            if (slot[e] < 0) continue;
-            const unsigned x = l.peak[slot[e]];
+            if (static_cast<int>(at[e]) >= 0 || at[e] == kFree) continue;
+            const unsigned s = at[e] - kSlot, x = l.peak[s];
             unsigned long long q;
             if (x == kExpInf) {                    // counts of NaN and of infinities
                 q = p[e] != p[e] ? 1ull << 32 : p[e] > 1.7976931348623157e308 ? 1ull : 0ull;
@@ -1414,8 +1415,8 @@ __global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops
                 const double scaled = ldexp(p[e], 51 + 1022 - static_cast<int>(x ? x : 1));
                 q = static_cast<unsigned long long>(__double_as_longlong(scaled + 4503599627370496.0)) & 0xfffffffffffffull;
             }
-            atomicAdd(reinterpret_cast<unsigned long long*>(&l.sum[slot[e]]), q);
-            slot[e] = -2;
+            atomicAdd(reinterpret_cast<unsigned long long*>(&l.sum[s]), q);
+            at[e] = kFree;
         }
         __syncthreads();
         // the groups' values, moved together; behind them the list so far
@@ -1686,7 +1687,8 @@ void launch_merge_t(const MergeArgs& a, int64_t rows, hipStream_t st) {
 int launch_merge(const MergeArgs& a, int64_t rows, hipStream_t st) {
     const int n = a.K * a.k;
     if (n <= 64) launch_merge_t<64, 1, 128, false>(a, rows, st);
-    else if (n <= 256) launch_merge_t<64, 4, 512, false>(a, rows, st);
+    else if (n <= 128) launch_merge_t<64, 2, 256, false>(a, rows, st);
+    else if (n <= 256) launch_merge_t<128, 2, 512, false>(a, rows, st);
     else if (n <= 512) launch_merge_t<256, 2, 1024, false>(a, rows, st);
     else if (n <= 1024) launch_merge_t<256, 4, 1024, true>(a, rows, st);
     else if (n <= 2048) launch_merge_t<512, 4, 1024, true>(a, rows, st);
