@@ -215,10 +215,23 @@ __device__ __forceinline__ Acc acc_block(Acc v, Acc* lds) {
     v = acc_wave<ENT>(v);
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
     __syncthreads();
-    Acc r = lds[0];
+    if constexpr (THREADS / kWave > 4) {           // the waves' sums in lanes, joined as lanes are
+        Acc r = lds[threadIdx.x % (THREADS / kWave)];
 #pragma unroll
-    for (int i = 1; i < THREADS / kWave; ++i) r = acc_join<ENT>(r, lds[i]);
-    return r;
+        for (int d = THREADS / kWave / 2; d > 0; d >>= 1) {
+            Acc o;
+            o.R = __shfl_xor(r.R, d);
+            o.s = __shfl_xor(r.s, d);
+            o.e = ENT ? __shfl_xor(r.e, d) : 0.0f;
+            r = acc_join<ENT>(r, o);
+        }
+        return r;
+    } else {
+        Acc r = lds[0];
+#pragma unroll
+        for (int i = 1; i < THREADS / kWave; ++i) r = acc_join<ENT>(r, lds[i]);
+        return r;
+    }
 }
 
 // What a row's softmax is afterwards.  slow: in terms of m and log s (natural, of (x - m) / T).
@@ -307,7 +320,9 @@ struct TopLds {
     static constexpr int kWaves = THREADS / kWave;
     static constexpr int kGroups = THREADS < 256 ? THREADS : 256;       // >= the largest `top`
     static constexpr int kRoom = kWaves == 16 ? 192 : 512;
+    static constexpr int kFlat = kWaves > 4 ? 512 : 0;
     uint64_t cand[kWaves * kRoom];
+    uint64_t flat[kFlat + 1];
     uint64_t list[kGroups];
     unsigned bound[kGroups];
     int held[kWaves];
@@ -434,34 +449,50 @@ __device__ __forceinline__ bool top_raise(TopLds<THREADS>& l, TopState<THREADS>&
     return fits;
 }
 
-// The candidates in order into l.list.  All threads; one barrier before, one after.
+// The candidates in order into l.list.  All threads; one barrier before (two with many waves), one after.
 template <int THREADS>
 __device__ __forceinline__ bool top_rank(TopLds<THREADS>& l, TopState<THREADS>& t, int top) {
     using L = TopLds<THREADS>;
+    constexpr int kStep = 8;                                     // reads on their way at once
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    auto count_above = [](const uint64_t* o, int n, uint64_t key) {      // o is padded with zeros, which rank below every key
+        int above = 0;
+        for (int j = 0; j < n; j += kStep) {
+            uint64_t other[kStep];
+#pragma unroll
+            for (int q = 0; q < kStep; ++q) other[q] = o[j + q];
+#pragma unroll
+            for (int q = 0; q < kStep; ++q) above += other[q] > key;
+        }
+        return above;
+    };
     if (lane == 0) l.held[wave] = t.held;
-    // zeros, which rank below every key, up to a multiple of kStep
-    constexpr int kStep = 8;
     if (lane < kStep && t.held + lane < (t.held + kStep - 1) / kStep * kStep && t.held + lane < L::kRoom) t.mine[t.held + lane] = 0;
     __syncthreads();
     bool fits = true;
+    int total = 0, before = 0;
 #pragma unroll
-    for (int w = 0; w < L::kWaves; ++w) fits = fits && l.held[w] <= L::kRoom;
-    if (fits) {
+    for (int w = 0; w < L::kWaves; ++w) {
+        const int n = l.held[w];
+        fits = fits && n <= L::kRoom;
+        before += w < wave ? n : 0;
+        total += n;
+    }
+    if (L::kFlat && fits && total <= L::kFlat - kStep) {         // many waves with few candidates each: side by side
+        if (lane < t.held) l.flat[before + lane] = t.mine[lane];
+        for (int i = lane + kWave; i < t.held; i += kWave) l.flat[before + i] = t.mine[i];
+        if (threadIdx.x < kStep) l.flat[total + threadIdx.x] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < total; i += THREADS) {
+            const uint64_t key = l.flat[i];
+            const int rank = count_above(l.flat, total, key);
+            if (rank < top) l.list[rank] = key;
+        }
+    } else if (fits) {
         for (int i = lane; i < t.held; i += kWave) {
             const uint64_t key = t.mine[i];
             int rank = 0;
-            for (int w = 0; w < L::kWaves; ++w) {
-                const int n = l.held[w];
-                const uint64_t* o = l.cand + w * L::kRoom;
-                for (int j = 0; j < n; j += kStep) {             // kStep reads on their way at once
-                    uint64_t other[kStep];
-#pragma unroll
-                    for (int q = 0; q < kStep; ++q) other[q] = o[j + q];
-#pragma unroll
-                    for (int q = 0; q < kStep; ++q) rank += other[q] > key;
-                }
-            }
+            for (int w = 0; w < L::kWaves; ++w) rank += count_above(l.cand + w * L::kRoom, l.held[w], key);
             if (rank < top) l.list[rank] = key;
         }
     }
@@ -626,6 +657,13 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
 #pragma unroll
     for (int u = 0; u < kU; ++u) cur[u] = next[u];
     if (kU * THREADS < sp.nvec) fetch(kU * THREADS);
+    // the target's logit, long before it is wanted
+    int64_t want = a.ignore_index;
+    float given = 0.0f;
+    if (tid == 0 && a.targets) {
+        want = a.targets[row];
+        if (want >= 0 && want < a.vocab) given = E::widen(x[want]);
+    }
     {
         const float v[2] = {head, tail};
         acc_add<true>(acc, v, fmaxf(head, tail), k);
@@ -739,10 +777,9 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
         a.lse[row] = lse;
         a.entropy[row] = st.entropy;
         if (a.targets) {
-            const int64_t want = a.targets[row];
             float lp = 0.0f;
             if (want != a.ignore_index)
-                lp = want >= 0 && want < a.vocab ? log_prob(st, a.scale, E::widen(x[want]), lse) : __builtin_nanf("");
+                lp = want >= 0 && want < a.vocab ? log_prob(st, a.scale, given, lse) : __builtin_nanf("");
             a.logprob[row] = lp;
         }
     }
