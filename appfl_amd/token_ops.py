@@ -210,20 +210,29 @@ class _Distill(torch.autograd.Function):
         if rc:
             N.check(rc, "fa_distill_loss")
         ctx.save_for_backward(logits, stat, *keep)
-        ctx.temperature = t.temperature
+        ctx.call = x, t, logits.stride(), t.id_stride, t.lp_stride
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, row_grad):
-        # pointers anew: hooks on saved tensors may hand back other memory than was saved
+        # Python costs three times as much in autograd's threads: the forward call's structures are used
+        # again, with pointers (and, if they changed, strides) anew, because hooks on saved tensors may
+        # hand back other memory than was saved.
         logits, stat, ids, logprobs, row_weight = ctx.saved_tensors
-        x = _logits(logits)
-        t = N.Teacher(ids.data_ptr(), logprobs.data_ptr(), ids.stride(0), logprobs.stride(0), _ptr(row_weight),
-                      ctx.temperature, ids.shape[-1])
+        x, t, strides, id_stride, lp_stride = ctx.call
+        if logits.stride() != strides or ids.stride(0) != id_stride or logprobs.stride(0) != lp_stride:
+            x = _logits(logits)
+            t = N.Teacher(None, None, ids.stride(0), logprobs.stride(0), None, t.temperature, t.k)
+        else:
+            x.data = logits.data_ptr()
+        t.ids, t.logprobs = ids.data_ptr(), logprobs.data_ptr()
+        if row_weight is not None:
+            t.row_weight = row_weight.data_ptr()
         index = logits.get_device()
         with _on(index):
-            row_grad = row_grad.contiguous()
+            if not row_grad.is_contiguous():
+                row_grad = row_grad.contiguous()
             grad = logits.new_empty(logits.shape)
             rc = N.load().fa_distill_grad(C.byref(x), C.byref(t), stat.data_ptr(), row_grad.data_ptr(), grad.data_ptr(),
                                           x.inner * x.vocab, x.vocab, _raw_stream(index))
