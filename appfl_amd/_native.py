@@ -40,7 +40,7 @@ class MeanSegment(C.Structure):
 
 FA_LOGITS_F32, FA_LOGITS_BF16, FA_LOGITS_F16 = range(3)
 FA_VOCAB_MAX, FA_DISTILL_STAT = 1 << 30, 4
-FA_TOP_MAX, FA_MERGE_CLIENTS, FA_MERGE_ENTRIES = 256, 128, 8192
+FA_TOP_MAX, FA_SCORES_TOP_MAX, FA_MERGE_CLIENTS, FA_MERGE_ENTRIES = 256, 128, 128, 8192
 
 
 class Logits(C.Structure):

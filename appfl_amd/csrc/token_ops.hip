@@ -45,8 +45,9 @@ template <> struct Elem<FA_LOGITS_F16> {
 
 struct Rows {            // a [outer, inner, vocab] view with unit stride along the vocabulary
     int64_t inner, stride_outer, stride_inner;
-    __device__ __forceinline__ int64_t offset(int64_t row) const {
-        return (row / inner) * stride_outer + (row % inner) * stride_inner;
+    __device__ __forceinline__ int64_t offset(int64_t row) const {       // rows and inner are below 2^31
+        const unsigned r = static_cast<unsigned>(row), n = static_cast<unsigned>(inner), o = r / n;
+        return o * stride_outer + (r - o * n) * stride_inner;
     }
 };
 
@@ -318,7 +319,7 @@ __device__ __forceinline__ float key_value(uint64_t key) {       // not for a Na
 template <int THREADS>
 struct TopLds {
     static constexpr int kWaves = THREADS / kWave;
-    static constexpr int kGroups = THREADS < 256 ? THREADS : 256;       // >= the largest `top`
+    static constexpr int kGroups = THREADS < 256 ? THREADS : 256;       // twice the largest `top`, so that the bound is near it
     static constexpr int kRoom = kWaves == 16 ? 192 : 512;
     static constexpr int kFlat = kWaves > 4 ? 512 : 0;
     uint64_t cand[kWaves * kRoom];
@@ -449,23 +450,27 @@ __device__ __forceinline__ bool top_raise(TopLds<THREADS>& l, TopState<THREADS>&
     return fits;
 }
 
+// How many of n keys are above `key`; kStep reads are on their way at once, so that the keys are padded
+// with zeros, which are below every key, to a multiple of it.
+constexpr int kStep = 8;
+
+__device__ __forceinline__ int count_above(const uint64_t* o, int n, uint64_t key) {
+    int above = 0;
+    for (int j = 0; j < n; j += kStep) {
+        uint64_t other[kStep];
+#pragma unroll
+        for (int q = 0; q < kStep; ++q) other[q] = o[j + q];
+#pragma unroll
+        for (int q = 0; q < kStep; ++q) above += other[q] > key;
+    }
+    return above;
+}
+
 // The candidates in order into l.list.  All threads; one barrier before (two with many waves), one after.
 template <int THREADS>
 __device__ __forceinline__ bool top_rank(TopLds<THREADS>& l, TopState<THREADS>& t, int top) {
     using L = TopLds<THREADS>;
-    constexpr int kStep = 8;                                     // reads on their way at once
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    auto count_above = [](const uint64_t* o, int n, uint64_t key) {      // o is padded with zeros, which rank below every key
-        int above = 0;
-        for (int j = 0; j < n; j += kStep) {
-            uint64_t other[kStep];
-#pragma unroll
-            for (int q = 0; q < kStep; ++q) other[q] = o[j + q];
-#pragma unroll
-            for (int q = 0; q < kStep; ++q) above += other[q] > key;
-        }
-        return above;
-    };
     if (lane == 0) l.held[wave] = t.held;
     if (lane < kStep && t.held + lane < (t.held + kStep - 1) / kStep * kStep && t.held + lane < L::kRoom) t.mine[t.held + lane] = 0;
     __syncthreads();
@@ -543,13 +548,17 @@ __device__ __forceinline__ void top_bound(TopLds<THREADS>& l, unsigned best, int
 template <int DT, int THREADS>
 __device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw* x, int vocab, int top, TopLds<THREADS>& l) {
     using L = TopLds<THREADS>;
+    constexpr int kElements = L::kGroups * 8;
     const int tid = threadIdx.x;
     int have = 0;
     uint64_t low = 0;                                            // the list's last key once it is full
-    constexpr int kStep = L::kGroups * 8;
-    for (int base = 0; base < vocab; base += kStep) {
+    for (int j = tid; j < L::kGroups; j += THREADS) l.list[j] = 0;
+    for (int base = 0; base < vocab; base += kElements) {
         __syncthreads();
-        if (tid == 0) l.count = 0;
+        if (tid == 0) {
+            l.count = 0;
+            l.reach = 0;
+        }
         uint64_t best = 0;
         uint64_t keys[8];
 #pragma unroll
@@ -562,13 +571,8 @@ __device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw*
         }
         // keys are all different, so at most 8 * top elements reach the top-th of the groups' best
         if (tid < L::kGroups) l.cand[tid] = best;
-        if (tid == 0) l.reach = 0;
         __syncthreads();
-        if (tid < L::kGroups && best) {
-            int rank = 0;
-            for (int j = 0; j < L::kGroups; ++j) rank += l.cand[j] > best;
-            if (rank == top - 1) l.reach = best;
-        }
+        if (tid < L::kGroups && best && count_above(l.cand, L::kGroups, best) == top - 1) l.reach = best;
         __syncthreads();
         const uint64_t reach = l.reach;
 #pragma unroll
@@ -576,6 +580,8 @@ __device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw*
             if (keys[j] && keys[j] >= reach) l.cand[atomicAdd(&l.count, 1u)] = keys[j];
         __syncthreads();
         const int n = static_cast<int>(l.count), total = have + n;
+        if (tid < kStep && n + tid < L::kWaves * L::kRoom) l.cand[n + tid] = 0;
+        __syncthreads();
         constexpr int kOwn = (8 * L::kGroups + L::kGroups + THREADS - 1) / THREADS;
         uint64_t own[kOwn];
         int rank[kOwn];
@@ -586,9 +592,7 @@ __device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw*
             rank[e] = top;
             if (i >= total) continue;
             own[e] = i < have ? l.list[i] : l.cand[i - have];
-            rank[e] = 0;
-            for (int j = 0; j < have; ++j) rank[e] += l.list[j] > own[e];
-            for (int j = 0; j < n; ++j) rank[e] += l.cand[j] > own[e];
+            rank[e] = (i < have ? i : count_above(l.list, have, own[e])) + count_above(l.cand, n, own[e]);
         }
         __syncthreads();
 #pragma unroll
@@ -610,6 +614,7 @@ struct ScoreArgs {
     float *logprob, *entropy, *lse, *top_logprobs;
     int32_t* top_ids;
     Scale scale;
+    int64_t row0;                // of the launch's first block
 };
 
 __device__ __forceinline__ float log_prob(const RowStat& st, const Scale& sc, float v, float lse) {
@@ -633,7 +638,7 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
     __shared__ Acc lds[THREADS / kWave];
     __shared__ float red[THREADS / kWave];
     __shared__ L l;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
     const Span sp = V::span(x, a.vocab);
     const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
@@ -726,14 +731,7 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
         t.floor = lim;           // `top` elements reach it; -inf without a bound, and there is no further chunk
     }
     bool fits = true;
-    // Chunks read when the floor is raised next.  The first chunk's bound is near the top-th element
-    // while `top` is well below the number of groups; beyond three quarters of it a wave's room would
-    // not last four chunks.
-    int chunk = 1, due = 4;
-    if (TOP && a.top > L::kGroups * 3 / 4) {
-        fits = top_raise(l, t, a.top);
-        due = 2;
-    }
+    int chunk = 1, due = 4;                                      // chunks read when the floor is raised next
     for (int base = kU * THREADS; base < sp.nvec; ++chunk) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) cur[u] = next[u];
@@ -815,6 +813,7 @@ struct DistillArgs {
     const float* row_grad;
     void* grad;
     Rows grad_rows;
+    int64_t row0;                // of the launch's first block
 };
 
 // One row's teacher, made by the first wave alone: entries j = lane + 64 i.
@@ -1085,7 +1084,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     __shared__ Acc lds[THREADS / kWave];
     __shared__ float red[THREADS / kWave];
     __shared__ TeacherLds l;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const int part = blockIdx.y, parts = gridDim.y;              // LOSS: one part
     const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
     const float weight = a.t.row_weight ? a.t.row_weight[row] : 1.0f;
@@ -1153,7 +1152,7 @@ __global__ __launch_bounds__(THREADS) void distill_step_kernel(const DistillArgs
     __shared__ Acc lds[THREADS / kWave];
     __shared__ float red[THREADS / kWave];
     __shared__ TeacherLds l;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
     typename E::Raw* g = static_cast<typename E::Raw*>(a.grad) + a.grad_rows.offset(row);
     const float weight = a.t.row_weight ? a.t.row_weight[row] : 1.0f;
@@ -1246,6 +1245,7 @@ struct MergeArgs {
     const float* unit;
     int64_t unit_client, unit_row;
     int K, k, top;
+    int64_t row0;                // of the launch's first block
     uint64_t per_k;              // 2^32 / k, rounded up: i / k for i * k < 2^32
     int32_t* out_ids;
     float* out_lp;
@@ -1349,7 +1349,7 @@ __global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops
     using L = MergeLds<SLOTS, ROUNDS>;
     constexpr int kGroupsPer = (SLOTS + THREADS - 1) / THREADS;
     __shared__ L l;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const int tid = threadIdx.x;
     const int n = a.K * a.k;
     // entry e of a thread is i = tid + e * THREADS = (client, place) = (i / k, i % k)
@@ -1622,7 +1622,7 @@ int check_teacher(const fa_teacher* t, int64_t rows) {
     if (!t || t->k < 1 || t->k > FA_TOP_MAX) return FA_ERR_INVALID;
     if (rows && (!t->ids || !t->logprobs)) return FA_ERR_INVALID;
     if (t->id_stride < 0 || t->lp_stride < 0) return FA_ERR_INVALID;
-    if (!(t->temperature > 0.0) || !(t->temperature <= 1e30) || !(t->temperature >= 1e-30)) return FA_ERR_INVALID;
+    if (!(t->temperature >= 1e-6) || !(t->temperature <= 1e6)) return FA_ERR_INVALID;
     return FA_OK;
 }
 
@@ -1653,10 +1653,23 @@ constexpr int64_t kMemoryCache = 256ll << 20;      // the last-level cache of th
 
 int64_t row_bytes(const fa_logits* x) { return static_cast<int64_t>(x->vocab) * elem_size(x->dtype); }
 
+// A launch counts its threads in 32 bits: 2^21 rows of up to 1024 threads at a time.
+constexpr int64_t kRowsPerLaunch = 1 << 21;
+
+template <class Args, class Launch>
+void for_rows(int64_t rows, Args a, Launch launch) {
+    for (a.row0 = 0; a.row0 < rows; a.row0 += kRowsPerLaunch) {
+        const int64_t left = rows - a.row0;
+        launch(static_cast<unsigned>(left < kRowsPerLaunch ? left : kRowsPerLaunch), a);
+    }
+}
+
 template <int DT, int THREADS, bool LOSS, bool GRAD, bool LAST>
-void launch_distill_t(int64_t rows, int parts, const DistillArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((distill_kernel<DT, THREADS, LOSS, GRAD, LAST>),
-                       dim3(static_cast<unsigned>(rows), static_cast<unsigned>(parts)), dim3(THREADS), 0, st, a);
+void launch_distill_t(int64_t rows, int parts, const DistillArgs& args, hipStream_t st) {
+    for_rows(rows, args, [&](unsigned n, const DistillArgs& a) {
+        hipLaunchKernelGGL((distill_kernel<DT, THREADS, LOSS, GRAD, LAST>), dim3(n, static_cast<unsigned>(parts)),
+                           dim3(THREADS), 0, st, a);
+    });
 }
 
 template <int DT>
@@ -1678,8 +1691,10 @@ void launch_grad(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
 }
 
 template <int DT, int NV>
-void launch_step_t(int64_t rows, const DistillArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((distill_step_kernel<DT, kWave, NV>), dim3(static_cast<unsigned>(rows)), dim3(kWave), 0, st, a);
+void launch_step_t(int64_t rows, const DistillArgs& args, hipStream_t st) {
+    for_rows(rows, args, [&](unsigned n, const DistillArgs& a) {
+        hipLaunchKernelGGL((distill_step_kernel<DT, kWave, NV>), dim3(n), dim3(kWave), 0, st, a);
+    });
 }
 
 template <int DT>
@@ -1699,12 +1714,13 @@ void launch_step(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
 }
 
 template <int DT, int THREADS>
-void launch_scores_t(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(x->outer * x->inner));
-    if (a.top)
-        hipLaunchKernelGGL((token_scores_kernel<DT, THREADS, true>), grid, dim3(THREADS), 0, st, a);
-    else
-        hipLaunchKernelGGL((token_scores_kernel<DT, THREADS, false>), grid, dim3(THREADS), 0, st, a);
+void launch_scores_t(const fa_logits* x, const ScoreArgs& args, hipStream_t st) {
+    for_rows(x->outer * x->inner, args, [&](unsigned n, const ScoreArgs& a) {
+        if (a.top)
+            hipLaunchKernelGGL((token_scores_kernel<DT, THREADS, true>), dim3(n), dim3(THREADS), 0, st, a);
+        else
+            hipLaunchKernelGGL((token_scores_kernel<DT, THREADS, false>), dim3(n), dim3(THREADS), 0, st, a);
+    });
 }
 
 template <int DT>
@@ -1721,9 +1737,10 @@ void launch_scores(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
 hipStream_t as_stream(fa_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 template <int THREADS, int PER, int SLOTS, bool ROUNDS>
-void launch_merge_t(const MergeArgs& a, int64_t rows, hipStream_t st) {
-    hipLaunchKernelGGL((merge_tops_kernel<THREADS, PER, SLOTS, ROUNDS>), dim3(static_cast<unsigned>(rows)), dim3(THREADS),
-                       0, st, a);
+void launch_merge_t(const MergeArgs& args, int64_t rows, hipStream_t st) {
+    for_rows(rows, args, [&](unsigned n, const MergeArgs& a) {
+        hipLaunchKernelGGL((merge_tops_kernel<THREADS, PER, SLOTS, ROUNDS>), dim3(n), dim3(THREADS), 0, st, a);
+    });
 }
 
 // Threads for at most 16 entries each; a table that holds every token of a short list at once.
@@ -1748,12 +1765,12 @@ int fa_token_scores(const fa_logits* x, const int64_t* targets, int64_t ignore_i
                     float* entropy, float* lse, int32_t* top_ids, float* top_logprobs, fa_stream_t stream) {
     const int rc = check_logits(x);
     if (rc != FA_OK) return rc;
-    if (top < 0 || top > FA_TOP_MAX || top > x->vocab) return FA_ERR_INVALID;
+    if (top < 0 || top > FA_SCORES_TOP_MAX || top > x->vocab) return FA_ERR_INVALID;
     const int64_t rows = x->outer * x->inner;
     if (rows == 0) return FA_OK;
     if (!entropy || !lse || (targets && !logprob) || (top && (!top_ids || !top_logprobs))) return FA_ERR_INVALID;
     const ScoreArgs a = {x->data, rows_of(x), x->vocab, top, targets, ignore_index, logprob, entropy, lse,
-                         top_logprobs, top_ids, scale_of(1.0)};
+                         top_logprobs, top_ids, scale_of(1.0), 0};
     switch (x->dtype) {
         case FA_LOGITS_F32: launch_scores<FA_LOGITS_F32>(x, a, as_stream(stream)); break;
         case FA_LOGITS_BF16: launch_scores<FA_LOGITS_BF16>(x, a, as_stream(stream)); break;

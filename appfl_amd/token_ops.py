@@ -117,8 +117,8 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, t
     index = logits.get_device()
     if type(top) is not int:
         raise TypeError("top must be an int")
-    if not 0 <= top <= min(TOP_MAX, x.vocab):
-        raise ValueError(f"top must be in 0..{min(TOP_MAX, x.vocab)}, got {top}")
+    if not 0 <= top <= min(N.FA_SCORES_TOP_MAX, x.vocab):
+        raise ValueError(f"top must be in 0..{min(N.FA_SCORES_TOP_MAX, x.vocab)}, got {top}")
     lead = logits.shape[:-1]
     logprob = ids = tops = None
     with _on(index):
@@ -185,8 +185,8 @@ def _teacher(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, te
     index = logits.get_device()
     k = _lists(ids, logprobs, index, lead)
     tau = float(temperature)
-    if not 1e-30 <= tau <= 1e30:
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= tau <= 1e6:
+        raise ValueError(f"temperature must be in 1e-6..1e6, got {temperature}")
     if row_weight is not None:
         _check("row_weight", row_weight, _f32, index, lead)
         row_weight = row_weight.contiguous()

@@ -500,6 +500,7 @@ enum { FA_LOGITS_F32 = 0, FA_LOGITS_BF16 = 1, FA_LOGITS_F16 = 2 };
 #define FA_VOCAB_MAX (1 << 30) /* tokens of a vocabulary                                      */
 #define FA_DISTILL_STAT 4      /* floats per row that fa_distill_loss leaves for the gradient */
 #define FA_TOP_MAX 256         /* entries of one list                                         */
+#define FA_SCORES_TOP_MAX 128  /* top entries of one fa_token_scores call                     */
 #define FA_MERGE_CLIENTS 128   /* clients of one fa_merge_tops call                           */
 #define FA_MERGE_ENTRIES 8192  /* clients * entries of one list of one fa_merge_tops call     */
 
@@ -515,7 +516,7 @@ typedef struct {             /* one list per row: entry j of row r at ids[r * id
     const float* logprobs;
     int64_t id_stride, lp_stride;
     const float* row_weight; /* one per row, packed; NULL: 1 */
-    double temperature;      /* in [1e-30, 1e30] */
+    double temperature;      /* in [1e-6, 1e6] */
     int k;                   /* 1..FA_TOP_MAX */
 } fa_teacher;
 
@@ -534,7 +535,7 @@ typedef struct {             /* entry j of client c's row r at ids[c * id_client
  *   vocabulary);  top_ids / top_logprobs: the `top` largest logits, best first, equal ones (and -0
  *   and +0) by the lower id first, NaN before everything.
  * A row of nothing but -inf has lse = -inf, entropy 0 and log probabilities of -inf.  targets and
- * logprob may both be NULL; 0 <= top <= min(vocab, FA_TOP_MAX).
+ * logprob may both be NULL; 0 <= top <= min(vocab, FA_SCORES_TOP_MAX).
  */
 int fa_token_scores(const fa_logits* logits, const int64_t* targets, int64_t ignore_index, int top,
                     float* logprob, float* entropy, float* lse, int32_t* top_ids,

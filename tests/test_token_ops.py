@@ -66,6 +66,9 @@ def test_outputs_and_null_pointers_are_checked():
     for change in (dict(entropy=None), dict(lse=None), dict(targets=256), dict(top=2), dict(top=2, ids=256), dict(top=11),
                    dict(top=-1)):
         assert scores(**change) == INVALID, change
+    x.vocab = 1000
+    assert scores(top=129, ids=256, lps=256) == INVALID
+    x.vocab = 10
     assert lib.fa_distill_loss(C.byref(x), None, 256, 256, None) == INVALID
     assert lib.fa_distill_loss(C.byref(x), C.byref(t), None, 256, None) == INVALID
     assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, None, None) == INVALID
