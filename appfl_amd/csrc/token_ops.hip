@@ -623,9 +623,10 @@ __device__ __forceinline__ float log_prob(const RowStat& st, const Scale& sc, fl
     return fabsf(y) < 1e30f ? y * sc.inv_k : v - lse;
 }
 
-// One block per row: kU vectors of 16 bytes per thread and chunk, the next chunk's loads in flight
-// while one is summed.
-constexpr int kU = 4;
+// One block per row: a few vectors of 16 bytes per thread and chunk, the next chunk's loads in flight
+// while one is summed.  Blocks of 256 threads take two: four need more than their 64 registers (fp32
+// 4096 x 128000, top 8: 314 us with two, 343 with four; 2048 x 50261 bf16, top 32: 55 and 57).
+constexpr int scores_vectors(int threads) { return threads == 256 ? 2 : 4; }
 
 // Blocks of 256 threads: eight fit a CU by their LDS (19.6 KiB), 64 registers a thread.
 constexpr int scores_waves(int threads, bool top) { return !top ? 1 : threads == 1024 ? 4 : threads == 256 ? 8 : 6; }
@@ -635,6 +636,7 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
     using E = Elem<DT>;
     using V = Vec<DT>;
     using L = TopLds<THREADS>;
+    constexpr int kU = scores_vectors(THREADS);
     __shared__ Acc lds[THREADS / kWave];
     __shared__ float red[THREADS / kWave];
     __shared__ L l;
@@ -977,6 +979,8 @@ __device__ __forceinline__ Softmax softmax_of(const RowStat& st, const Scale& sc
     f.c = c;
     return f;
 }
+
+constexpr int kU = 4;      // vectors a thread has on their way
 
 // Writes f(element) over elements [lo, hi) of a row; reads by 16 bytes, writes so where the
 // gradient's row has the same alignment.
