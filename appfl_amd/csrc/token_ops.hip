@@ -319,7 +319,10 @@ __device__ __forceinline__ float key_value(uint64_t key) {       // not for a Na
 template <int THREADS>
 struct TopLds {
     static constexpr int kWaves = THREADS / kWave;
-    static constexpr int kGroups = THREADS < 256 ? THREADS : 256;       // twice the largest `top`, so that the bound is near it
+    // groups for the first chunk's bound: twice the largest `top`, so that the bound is near it.  A lone
+    // wave's lanes make two each, of their even and their odd vectors.
+    static constexpr int kGroups = THREADS == kWave ? 128 : 256;
+    static constexpr int kSplit = THREADS == kWave ? 2 : 1;
     static constexpr int kRoom = kWaves == 16 ? 192 : 512;
     static constexpr int kFlat = kWaves > 4 ? 512 : 0;
     uint64_t cand[kWaves * kRoom];
@@ -330,7 +333,7 @@ struct TopLds {
     float floor[kWaves];
     unsigned limit, limit_group, tie, count;
     uint64_t reach;
-    static_assert(kWaves * kRoom >= kGroups * 8, "a step of slow_top");
+    static_assert(kWaves * kRoom >= (kGroups < THREADS ? kGroups : THREADS) * 8, "a step of slow_top");
 };
 
 __device__ __forceinline__ unsigned order_of(float v) { return static_cast<unsigned>(order_key(v, 0) >> 32); }
@@ -505,15 +508,19 @@ __device__ __forceinline__ bool top_rank(TopLds<THREADS>& l, TopState<THREADS>& 
     return fits;
 }
 
-// The first chunk's bound.  `best`: the caller's largest element as order_of (0: none).  Afterwards
-// l.limit is the bound (0: fewer than `top` groups have an element) and l.limit_group the last group
-// whose equal elements are needed (all of them: INT32_MAX).
+// The first chunk's bound.  `best`: the largest element of the caller's groups (or of the group of kShare
+// neighbours it is in) as order_of, 0: none.  Afterwards l.limit is the bound (0: fewer than `top` groups
+// have an element) and l.limit_group the last group whose equal elements are needed (all: INT32_MAX).
+// Group h of a thread is h * kWave + thread, or thread / kShare.
 template <int THREADS>
-__device__ __forceinline__ void top_bound(TopLds<THREADS>& l, unsigned best, int top) {
+__device__ __forceinline__ void top_bound(TopLds<THREADS>& l, const unsigned (&best)[TopLds<THREADS>::kSplit], int top) {
     using L = TopLds<THREADS>;
-    constexpr int kShare = THREADS / L::kGroups, kRegs = L::kGroups / kWave;
+    constexpr int kShare = THREADS * L::kSplit / L::kGroups, kRegs = L::kGroups / kWave;
     const int tid = threadIdx.x;
-    if (tid % kShare == 0) l.bound[tid / kShare] = best;
+    if (tid % kShare == 0) {
+#pragma unroll
+        for (int h = 0; h < L::kSplit; ++h) l.bound[h * kWave + tid / kShare] = best[h];
+    }
     __syncthreads();
     if (tid < kWave) {
         unsigned v[kRegs];
@@ -544,11 +551,11 @@ __device__ __forceinline__ void top_bound(TopLds<THREADS>& l, unsigned best, int
     __syncthreads();
 }
 
-// Steps of 8 elements per group; exact for every row, NaN included.
+// Steps of 8 elements a thread, 256 threads at most; exact for every row, NaN included.
 template <int DT, int THREADS>
 __device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw* x, int vocab, int top, TopLds<THREADS>& l) {
     using L = TopLds<THREADS>;
-    constexpr int kElements = L::kGroups * 8;
+    constexpr int kTakers = L::kGroups < THREADS ? L::kGroups : THREADS, kElements = kTakers * 8;
     const int tid = threadIdx.x;
     int have = 0;
     uint64_t low = 0;                                            // the list's last key once it is full
@@ -564,15 +571,15 @@ __device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw*
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = base + tid * 8 + j;
-            const bool in = tid < L::kGroups && i < vocab;
+            const bool in = tid < kTakers && i < vocab;
             keys[j] = in ? order_key(Elem<DT>::widen(x[i]), i) : 0;
             if (keys[j] <= low) keys[j] = 0;
             best = keys[j] > best ? keys[j] : best;
         }
-        // keys are all different, so at most 8 * top elements reach the top-th of the groups' best
-        if (tid < L::kGroups) l.cand[tid] = best;
+        // keys are all different, so at most 8 * top elements reach the top-th of the threads' best
+        if (tid < kTakers) l.cand[tid] = best;
         __syncthreads();
-        if (tid < L::kGroups && best && count_above(l.cand, L::kGroups, best) == top - 1) l.reach = best;
+        if (tid < kTakers && best && count_above(l.cand, kTakers, best) == top - 1) l.reach = best;
         __syncthreads();
         const uint64_t reach = l.reach;
 #pragma unroll
@@ -582,7 +589,7 @@ __device__ __attribute__((noinline)) void slow_top(const typename Elem<DT>::Raw*
         const int n = static_cast<int>(l.count), total = have + n;
         if (tid < kStep && n + tid < L::kWaves * L::kRoom) l.cand[n + tid] = 0;
         __syncthreads();
-        constexpr int kOwn = (8 * L::kGroups + L::kGroups + THREADS - 1) / THREADS;
+        constexpr int kOwn = (kElements + L::kGroups + THREADS - 1) / THREADS;
         uint64_t own[kOwn];
         int rank[kOwn];
 #pragma unroll
@@ -675,21 +682,28 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
         const float v[2] = {head, tail};
         acc_add<true>(acc, v, fmaxf(head, tail), k);
     }
-    float most = head;
+    float most[L::kSplit];
+    most[0] = head;
+#pragma unroll
+    for (int h = 1; h < L::kSplit; ++h) most[h] = -kInf;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
         float v[V::N];
         V::widen(cur[u], v);
         const float peak = V::peak(cur[u], v);
-        most = fmaxf(most, peak);
+        most[u % L::kSplit] = fmaxf(most[u % L::kSplit], peak);
         acc_add<true>(acc, v, peak, k);
     }
     if (TOP) {
-        constexpr int kShare = THREADS / L::kGroups;
-        unsigned best = tid < sp.head || tid < sp.nvec ? order_of(most) : 0;
-        for (int d = 1; d < kShare; d <<= 1) {
-            const unsigned o = __shfl_xor(best, d);
-            best = o > best ? o : best;
+        constexpr int kShare = THREADS * L::kSplit / L::kGroups;
+        unsigned best[L::kSplit];
+#pragma unroll
+        for (int h = 0; h < L::kSplit; ++h) {
+            best[h] = (h == 0 && tid < sp.head) || h * THREADS + tid < sp.nvec ? order_of(most[h]) : 0;
+            for (int d = 1; d < kShare; d <<= 1) {
+                const unsigned o = __shfl_xor(best[h], d);
+                best[h] = o > best[h] ? o : best[h];
+            }
         }
         top_bound(l, best, a.top);
         const unsigned limit = l.limit, last = l.limit_group;
@@ -697,10 +711,12 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
         int tie = INT32_MAX;
         if (last != INT32_MAX) {
             // groups up to `last` at the bound's value: the lowest index of each has to be let in
-            if (best == limit && static_cast<unsigned>(tid / kShare) <= last) {
-                int at = tid < sp.head && head == lim ? tid : INT32_MAX;
 #pragma unroll
-                for (int u = 0; u < kU; ++u) {
+            for (int h = 0; h < L::kSplit; ++h) {
+                if (best[h] != limit || static_cast<unsigned>(h * kWave + tid / kShare) > last) continue;
+                int at = h == 0 && tid < sp.head && head == lim ? tid : INT32_MAX;
+#pragma unroll
+                for (int u = h; u < kU; u += L::kSplit) {
                     float v[V::N];
                     V::widen_again(cur[u], v);
 #pragma unroll
@@ -1729,8 +1745,8 @@ void launch_scores_t(const fa_logits* x, const ScoreArgs& args, hipStream_t st) 
 
 template <int DT>
 void launch_scores(const fa_logits* x, const ScoreArgs& a, hipStream_t st) {
-    // a short row is one wave's: no barriers (its first chunk bounds up to 64 entries)
-    if (x->vocab <= 4096 && a.top <= kWave / 2)
+    // a short row is one wave's: no barriers (8192 x 1000 fp32, top 64: 27 us, 44 with 256 threads)
+    if (x->vocab <= 4096 && a.top <= kWave)
         launch_scores_t<DT, kWave>(x, a, st);
     else if (wide_blocks(x->outer * x->inner, x->vocab))
         launch_scores_t<DT, 1024>(x, a, st);
