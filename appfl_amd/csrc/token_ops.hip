@@ -1,8 +1,16 @@
 // token_ops.hip -- operators on a language model's (or classifier's) answers, for federations that
 // exchange answers instead of weights: scoring a row of logits (log probability of the given token,
 // entropy, most probable tokens), merging K clients' top lists into one teacher, and distilling from
-// such lists (loss and gradient).  Softmax statistics are fp32 with the running maximum subtracted
-// first; merged probabilities are fp64 (their order decides which tokens are kept).
+// such lists (loss and gradient).
+//
+// Softmax sums are fp32 (below), lists are ranked by whole keys, merged probabilities are fp64 terms
+// added as 64-bit whole numbers (their order decides which tokens are kept).  Nothing is rounded to 16
+// bits but a gradient's elements, once.  A block takes a row; blocks share nothing, there is no
+// workspace, and no float is added atomically, so results are the same in every run.
+//
+// What bounds them (one MI355X): scores and the gradient alone move 5.0-6.9 TB/s of their bytes (8192 x
+// 128000 bf16: lists of 8 351 us, sums alone 322; a gradient 855 us), loss and gradient in one call
+// 4.5-4.9 TB/s counting the logits once (855-925 us); merges are bound by instructions and LDS latency.
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -310,12 +318,12 @@ __device__ __forceinline__ float key_value(uint64_t key) {       // not for a Na
 // elements reach, and the elements that reach it become candidates, in a buffer of their wave.  From
 // then on only elements above the floor -- a value that `top` elements before them reach -- are
 // candidates (an equal one has a higher index), found by comparing the largest of a vector's elements.
-// The floor is raised when 4, 8, 16, ... chunks have been read (2, 4, 8, ... cost 3 % more at 2048 x 50261) and at the end: with W waves, the least of the waves'
-// ceil(top / W)-th largest candidates.  Candidates below it are dropped; in a row in no particular
-// order about top * (1 + ln(n / chunk)) elements ever become candidates.  The last ones are ranked
-// against each other.
+// The floor is raised when 4, 8, 16, ... chunks have been read (2, 4, 8, ... cost 3 % more at
+// 2048 x 50261) and at the end: with W waves, to the least of the waves' ceil(top / W)-th largest
+// candidates.  Candidates below it are dropped; in a row in no particular order about
+// top * (1 + ln(n / chunk)) elements ever become candidates.  The last ones are ranked against each other.
 // A row that brings more candidates than fit (an ascending one) or holds a NaN is taken again by
-// slow_top, whose steps bring at most 8 * top.
+// slow_top, whose steps bring at most 8 * top: 2048 x 50261 bf16, top 32: 55 us, ascending 1.6 ms.
 template <int THREADS>
 struct TopLds {
     static constexpr int kWaves = THREADS / kWave;
@@ -1042,6 +1050,13 @@ __device__ __forceinline__ void map_row(const typename Elem<DT>::Raw* x, typenam
     }
 }
 
+// All of the block's stores have arrived before any thread goes on: the next store to one of their
+// addresses, by another wave, is the one that stays.
+__device__ __forceinline__ void stores_done() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0) alone
+    __syncthreads();
+}
+
 // The teacher's tokens, after the row's (or part's) other elements have been written: c (q - t).
 template <int DT>
 __device__ __forceinline__ void fix_row(typename Elem<DT>::Raw* g, const TeacherLds& l, int k, int lo, int hi, const Softmax& f) {
@@ -1097,7 +1112,7 @@ __device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int voca
 
 // LOSS alone: the sums of a row.  GRAD alone: from the sums of an earlier call; a row may be cut in
 // parts (blockIdx.y).  Both: the row is read twice, the second time from the memory-side cache as long
-// as the rows under way fit there (see step_threads).
+// as the rows under way fit there (see launch_step).
 template <int DT, int THREADS, bool LOSS, bool GRAD, bool LAST>
 __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     using E = Elem<DT>;
@@ -1154,7 +1169,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     }
     const Softmax f = softmax_of(st, a.scale, c);
     map_row<DT, THREADS, LAST>(x, g, a.vocab, part, parts, f);
-    __syncthreads();
+    stores_done();
     if (first_wave) {
         const Span sp = Vec<DT>::span(x, a.vocab);
         const int lo = part == 0 ? 0 : sp.head + static_cast<int>(static_cast<int64_t>(sp.nvec) * part / parts) * Vec<DT>::N;
@@ -1245,7 +1260,7 @@ __global__ __launch_bounds__(THREADS) void distill_step_kernel(const DistillArgs
         }
     }
     if (flat) return;
-    __syncthreads();
+    stores_done();
     if (first_wave) fix_row<DT>(g, l, a.t.k, 0, a.vocab, f);
 }
 
@@ -1642,7 +1657,7 @@ int check_teacher(const fa_teacher* t, int64_t rows) {
     if (!t || t->k < 1 || t->k > FA_TOP_MAX) return FA_ERR_INVALID;
     if (rows && (!t->ids || !t->logprobs)) return FA_ERR_INVALID;
     if (t->id_stride < 0 || t->lp_stride < 0) return FA_ERR_INVALID;
-    if (!(t->temperature >= 1e-6) || !(t->temperature <= 1e6)) return FA_ERR_INVALID;
+    if (!(t->temperature >= 1e-3) || !(t->temperature <= 1e3)) return FA_ERR_INVALID;
     return FA_OK;
 }
 

@@ -156,7 +156,10 @@ def merge_tops(ids: torch.Tensor, logprobs: torch.Tensor, weights: Sequence[floa
     if not 1 <= K <= N.FA_MERGE_CLIENTS or K * k > N.FA_MERGE_ENTRIES:
         raise ValueError(f"one merge takes 1..{N.FA_MERGE_CLIENTS} clients and {N.FA_MERGE_ENTRIES} entries a row, "
                          f"got {K} clients of {k}")
-    w = N.double_array(weights)
+    try:
+        w = N.double_array(weights)
+    except TypeError:                        # 0-d tensors, other libraries' numbers
+        w = N.double_array([float(v) for v in weights])
     if not all(0.0 <= v < math.inf for v in w):
         raise ValueError("client weights must be finite and not negative")
     if type(top) is not int:
@@ -185,8 +188,8 @@ def _teacher(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, te
     index = logits.get_device()
     k = _lists(ids, logprobs, index, lead)
     tau = float(temperature)
-    if not 1e-6 <= tau <= 1e6:
-        raise ValueError(f"temperature must be in 1e-6..1e6, got {temperature}")
+    if not 1e-3 <= tau <= 1e3:
+        raise ValueError(f"temperature must be in 1e-3..1e3, got {temperature}")
     if row_weight is not None:
         _check("row_weight", row_weight, _f32, index, lead)
         row_weight = row_weight.contiguous()

@@ -516,7 +516,7 @@ typedef struct {             /* one list per row: entry j of row r at ids[r * id
     const float* logprobs;
     int64_t id_stride, lp_stride;
     const float* row_weight; /* one per row, packed; NULL: 1 */
-    double temperature;      /* in [1e-6, 1e6] */
+    double temperature;      /* in [1e-3, 1e3] */
     int k;                   /* 1..FA_TOP_MAX */
 } fa_teacher;
 
@@ -565,7 +565,8 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
  * data and strides).  The gradient has the logits' type and row shape, with strides of its own;
  * its rows must not overlap.  A row with weight 0 or without an entry of probability above 0 has
  * loss and gradient 0 whatever its logits hold; an id >= vocab makes its row's loss and gradient
- * NaN.  A logit of -inf has q = 0 (loss inf where the teacher wants it).
+ * NaN.  A logit of -inf has q = 0 (loss inf where the teacher wants it).  Log probabilities are
+ * fp32, off by some 2^-20: the loss by T^2 times that.
  */
 int fa_distill_loss(const fa_logits* logits, const fa_teacher* teacher, float* loss, float* stat,
                     fa_stream_t stream);

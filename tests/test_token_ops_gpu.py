@@ -163,7 +163,7 @@ def check_distill(x, ids, lp, tau, weight=None, row_grad=None, view=None):
 @pytest.mark.parametrize("rows,vocab,k,tau", [
     (1, 1, 1, 1.0), (3, 2, 1, 2.0), (4, 10, 4, 2.0), (7, 63, 63, 1.0), (3, 64, 5, 0.5), (5, 129, 64, 1.5),
     (2, 257, 256, 1.0), (9, 1000, 32, 4.0), (3, 4099, 128, 1.0), (2, 16383, 16, 2.0), (3, 32003, 32, 1.0),
-    (2, 50261, 64, 2.0), (1, 131073, 8, 1.0), (2, 200003, 9, 3.0), (530, 1001, 3, 1.0)])
+    (2, 50261, 64, 2.0), (3, 777, 9, 1e-3), (3, 777, 9, 1e3), (1, 131073, 8, 1.0), (2, 200003, 9, 3.0), (530, 1001, 3, 1.0)])
 def test_distill(rows, vocab, k, tau, dtype):
     ids, lp = teacher(rows, vocab, k, seed=rows)
     check_distill(logits(rows, vocab, dtype, seed=vocab), ids, lp, tau)
@@ -336,7 +336,7 @@ def test_merge_ties_go_to_the_lowest_id():
     ids = torch.tensor([[[9, 4, 7, 1]], [[4, 9, 2, 7]]], dtype=torch.int32)
     lp = torch.full((2, 1, 4), -2.0)
     check_merge(ids, lp, [0.5, 0.5], 5)
-    got, _ = ops().merge_tops(ids.cuda(), lp.cuda(), [0.5, 0.5], 5)
+    got, _ = ops().merge_tops(ids.cuda(), lp.cuda(), torch.tensor([0.5, 0.5]), 5)
     assert got.cpu().tolist() == [[4, 7, 9, 1, 2]]
 
 
