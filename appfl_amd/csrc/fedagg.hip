@@ -174,8 +174,12 @@ __device__ __forceinline__ float optimizer_step(float step, float& m, float& v, 
     } else if (OPT == FA_OPT_YOGI) {
         float sg = sign_f32(v - s2);
         float yu = s2 * sg;
-        float ys = yu * h.omb2;
-        v = v - ys;
+        // v - yu * omb2, with the sign in the factor: v_sub_f32 turns the sign of a NaN it subtracts, the
+        // x86 subtraction PyTorch's results come from does not.  (Opaque: the compiler would subtract again.)
+        float neg = -h.omb2;
+        asm("" : "+s"(neg));
+        float ys = yu * neg;
+        v = v + ys;
     } else {  // FA_OPT_ADAGRAD
         v = v + s2;
     }
