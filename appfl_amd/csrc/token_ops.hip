@@ -1294,22 +1294,24 @@ __device__ __forceinline__ bool before(uint64_t ka, unsigned ia, uint64_t kb, un
 constexpr unsigned kFree = ~0u;
 constexpr unsigned kExpInf = 2047;
 
-// ROUNDS: rows may hold more different tokens than the table takes.
+// ROUNDS: rows may hold more different tokens than the table takes; else at most SLOTS / 2.
 template <int SLOTS, bool ROUNDS>
 struct MergeLds {
     static constexpr int kFull = SLOTS * 3 / 4;
     static constexpr int kList = ROUNDS ? FA_TOP_MAX : 0;
     static constexpr int kAll = SLOTS + kList + 8;
-    static constexpr int kBest = SLOTS < FA_TOP_MAX ? SLOTS : FA_TOP_MAX;
+    static_assert(!ROUNDS || SLOTS / 2 >= FA_TOP_MAX, "the ranked values");
     double share[FA_MERGE_CLIENTS];
     unsigned answered[FA_MERGE_CLIENTS];
     unsigned token[kAll];                          // by slot: id, ~0: free.  Later by group: id
     uint64_t sum[kAll];                            // by slot: sum.  Later by group: the value's bits
-    unsigned peak[SLOTS];                          // exponent of the group's largest term
-    u16 slot[SLOTS];                               // by group, in the order of their coming
+    union {
+        unsigned peak[SLOTS];                      // exponent of the group's largest term
+        uint64_t best[SLOTS / 2];                  // after the last round: the ranked values
+    };
+    u16 slot[ROUNDS ? SLOTS : SLOTS / 2];          // by group, in the order of their coming
     uint64_t list_key[kList + 1];                  // the best of the rounds before
     unsigned list_id[kList + 1];
-    uint64_t best[kBest];                          // the ranked values
     unsigned count, open, left, bound;
     double total;
 };
@@ -1352,7 +1354,7 @@ __device__ __forceinline__ int take_slot(MergeLds<SLOTS, ROUNDS>& l, unsigned id
 __device__ __forceinline__ unsigned exponent_of(double p) { return static_cast<unsigned>(__double2hiint(p)) >> 20 & 2047u; }
 
 // Waves a SIMD holds, so that the compiler keeps to their registers: as many as LDS lets in.
-constexpr int merge_waves(int threads, int per) { return per >= 8 ? 4 : threads == 256 && per == 4 ? 5 : 6; }
+constexpr int merge_waves(int threads, int per) { return per >= 8 ? 4 : threads == 256 ? (per == 4 ? 5 : 8) : 6; }
 
 // e^v of an fp32 value in fp64: 2^n times the Taylor series of e^r, |r| <= ln 2 / 2, whose first
 // omitted term is below 2^-57; log2(e) in two parts keeps r exact to fp64.  About half the
