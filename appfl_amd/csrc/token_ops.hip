@@ -1281,6 +1281,7 @@ struct MergeArgs {
     int64_t unit_client, unit_row;
     int K, k, top;
     int64_t row0;                // of the launch's first block
+    int near;                    // both lists have one client stride, K of which stay below 2^30 elements
     uint64_t per_k;              // 2^32 / k, rounded up: i / k for i * k < 2^32
     int32_t* out_ids;
     float* out_lp;
@@ -1396,20 +1397,37 @@ __global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops
     float lp[PER];
     {
         int j = tid - c0 * a.k;
-        const int32_t* ip = a.ids + row * a.id_row + c0 * a.id_client + j;
-        const float* lpp = a.lp + row * a.lp_row + c0 * a.lp_client + j;
-        const int64_t id_step = dc * a.id_client + dj, id_wrap = a.id_client - a.k;
-        const int64_t lp_step = dc * a.lp_client + dj, lp_wrap = a.lp_client - a.k;
+        if (a.near) {                              // one 32-bit offset serves both lists
+            const int32_t* ip = a.ids + row * a.id_row;
+            const float* lpp = a.lp + row * a.lp_row;
+            const unsigned client = static_cast<unsigned>(a.id_client), step = dc * client + dj, wrapped = client - a.k;
+            unsigned off = c0 * client + j;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            const bool in = tid + e * THREADS < n;
-            id[e] = in ? static_cast<unsigned>(*ip) : kFree;
-            lp[e] = in ? *lpp : 0.0f;
-            j += dj;
-            const bool wrap = j >= a.k;
-            j -= wrap ? a.k : 0;
-            ip += id_step + (wrap ? id_wrap : 0);
-            lpp += lp_step + (wrap ? lp_wrap : 0);
+            for (int e = 0; e < PER; ++e) {
+                const bool in = tid + e * THREADS < n;
+                id[e] = in ? static_cast<unsigned>(ip[off]) : kFree;
+                lp[e] = in ? lpp[off] : 0.0f;
+                j += dj;
+                const bool wrap = j >= a.k;
+                j -= wrap ? a.k : 0;
+                off += step + (wrap ? wrapped : 0);
+            }
+        } else {
+            const int32_t* ip = a.ids + row * a.id_row + c0 * a.id_client + j;
+            const float* lpp = a.lp + row * a.lp_row + c0 * a.lp_client + j;
+            const int64_t id_step = dc * a.id_client + dj, id_wrap = a.id_client - a.k;
+            const int64_t lp_step = dc * a.lp_client + dj, lp_wrap = a.lp_client - a.k;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const bool in = tid + e * THREADS < n;
+                id[e] = in ? static_cast<unsigned>(*ip) : kFree;
+                lp[e] = in ? *lpp : 0.0f;
+                j += dj;
+                const bool wrap = j >= a.k;
+                j -= wrap ? a.k : 0;
+                ip += id_step + (wrap ? id_wrap : 0);
+                lpp += lp_step + (wrap ? lp_wrap : 0);
+            }
         }
     }
     for (int c = tid; c < a.K; c += THREADS) {
@@ -1899,6 +1917,7 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
     a.K = K;
     a.k = in->k;
     a.top = top;
+    a.near = in->id_client == in->lp_client && in->id_client < (1 << 30) / K;
     a.per_k = ((1ull << 32) + in->k - 1) / in->k;
     a.out_ids = out_ids;
     a.out_lp = out_logprobs;

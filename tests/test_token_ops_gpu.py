@@ -361,6 +361,35 @@ def test_merge_of_strided_lists():
     assert torch.equal(got.cpu(), want.expand(rows, 4))
 
 
+def test_merge_of_lists_with_strides_of_their_own():
+    K, rows, k = 3, 11, 5
+    ids, lp = answers(K, rows, k, 20, seed=6)
+    for wide in (torch.int32, torch.float32):         # the ids' or the values' lists lie wider
+
+        def spread(t):
+            if t is None or t.dtype != wide:
+                return None if t is None else t.cuda()
+            big = torch.zeros(K, rows + 2, k, dtype=t.dtype, device="cuda")
+            big[:, 1:1 + rows] = t.cuda()
+            return big[:, 1:1 + rows]
+        check_merge(ids, lp, [1.0, 2.0, 0.5], 9, dev=spread)
+
+
+@pytest.mark.parametrize("client", [2**30 // 3 - 1, 2**30 // 3, 2**31 + 5])
+def test_merge_of_clients_far_apart(client):
+    K, rows, k = 3, 4, 5
+    ids, lp = answers(K, rows, k, 20, seed=7)
+
+    def spread(t):
+        if t is None:
+            return None
+        big = torch.empty((K - 1) * client + rows * k, dtype=t.dtype, device="cuda")
+        view = big.as_strided((K, rows, k), (client, k, 1))
+        view.copy_(t)
+        return view
+    check_merge(ids, lp, [1.0, 2.0, 0.5], 9, dev=spread)
+
+
 def test_more_rows_than_a_launch_takes():
     """Two classes, 2^22 + 3 rows: rows beyond the first launch's, against torch in 64 bits.
 
