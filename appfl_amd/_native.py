@@ -40,6 +40,7 @@ class MeanSegment(C.Structure):
 
 FA_LOGITS_F32, FA_LOGITS_BF16, FA_LOGITS_F16 = range(3)
 FA_VOCAB_MAX, FA_DISTILL_STAT = 1 << 30, 4
+FA_DISTILL_WS_ROWS, FA_DISTILL_WS_BYTES, FA_DISTILL_WS_FLOATS = 128, 204800, 2048
 FA_TOP_MAX, FA_SCORES_TOP_MAX, FA_MERGE_CLIENTS, FA_MERGE_ENTRIES = 256, 128, 128, 8192
 
 
@@ -135,7 +136,7 @@ SIGNATURES = {
     "fa_merge_tops": (_i, [_p, _p, _i, C.c_int64, _i, _p, _p, _p]),
     "fa_distill_loss": (_i, [_p, _p, _p, _p, _p]),
     "fa_distill_grad": (_i, [_p, _p, _p, _p, _p, C.c_int64, C.c_int64, _p]),
-    "fa_distill_loss_grad": (_i, [_p, _p, _p, _p, C.c_int64, C.c_int64, _p]),
+    "fa_distill_loss_grad": (_i, [_p, _p, _p, _p, C.c_int64, C.c_int64, _p, _p]),
     "fa_pack_host": (_i, [_p, _p, _p, _p, _i, _i]),
     "fa_pack_host_window": (_i, [_p, _p, _p, _p, _i, _sz, _sz, _i]),
     "fa_host_copy_fresh": (_i, [_p, _p, _sz, _i]),

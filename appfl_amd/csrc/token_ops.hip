@@ -835,6 +835,7 @@ struct DistillArgs {
     Scale scale;
     float* loss;
     float* stat;                 // FA_DISTILL_STAT floats per row: R, s, m, log s; R is NaN for a slow row
+    float* partial;              // FA_DISTILL_WS_FLOATS for the sums of rows' parts, or NULL
     const float* stat_in;
     const float* row_grad;
     void* grad;
@@ -1006,8 +1007,18 @@ __device__ __forceinline__ Softmax softmax_of(const RowStat& st, const Scale& sc
 
 constexpr int kU = 4;      // vectors a thread has on their way
 
-// Writes f(element) over elements [lo, hi) of a row; reads by 16 bytes, writes so where the
-// gradient's row has the same alignment.
+// Vectors [lo, hi) of a row's part; the head goes with the first part, the tail with the last.
+struct Part {
+    int lo, hi;
+};
+
+__device__ __forceinline__ Part part_of(const Span& sp, int part, int parts) {
+    return {static_cast<int>(static_cast<int64_t>(sp.nvec) * part / parts),
+            static_cast<int>(static_cast<int64_t>(sp.nvec) * (part + 1) / parts)};
+}
+
+// Writes f(element) over a part of a row; reads by 16 bytes, writes so where the gradient's row has
+// the same alignment.
 // LAST: the elements are read past the caches.
 template <int DT, int THREADS, bool LAST, class F>
 __device__ __forceinline__ void map_row(const typename Elem<DT>::Raw* x, typename Elem<DT>::Raw* g, int vocab, int part,
@@ -1023,8 +1034,7 @@ __device__ __forceinline__ void map_row(const typename Elem<DT>::Raw* x, typenam
     }
     const bool same = reinterpret_cast<uintptr_t>(x) % 16 == reinterpret_cast<uintptr_t>(g) % 16;
     const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
-    const int lo = static_cast<int>(static_cast<int64_t>(sp.nvec) * part / parts);
-    const int hi = static_cast<int>(static_cast<int64_t>(sp.nvec) * (part + 1) / parts);
+    const int lo = part_of(sp, part, parts).lo, hi = part_of(sp, part, parts).hi;
     for (int base = lo; base < hi; base += kU * THREADS) {
         uint4 r[kU];
 #pragma unroll
@@ -1067,39 +1077,37 @@ __device__ __forceinline__ void fix_row(typename Elem<DT>::Raw* g, const Teacher
 }
 
 template <int DT, int THREADS>
-__device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int vocab, float k) {
+__device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int vocab, float k, int part, int parts) {
     using E = Elem<DT>;
     using V = Vec<DT>;
     const Span sp = V::span(x, vocab);
     const int tid = threadIdx.x;
+    const int lo = part_of(sp, part, parts).lo, hi = part_of(sp, part, parts).hi;
     const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
     Acc acc = acc_empty();
-    if (tid < sp.head) {
+    uint4 next[kU];
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int i = base + u * THREADS + tid;
+            next[u] = i < hi ? body[i] : V::fill();
+        }
+    };
+    fetch(lo);
+    if (part == 0 && tid < sp.head) {
         const float v[1] = {E::widen(x[tid])};
         acc_add<false>(acc, v, v[0], k);
     }
-    if (tid < sp.tail) {
+    if (part == parts - 1 && tid < sp.tail) {
         const float v[1] = {E::widen(x[vocab - sp.tail + tid])};
         acc_add<false>(acc, v, v[0], k);
     }
-    uint4 next[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-        const int i = u * THREADS + tid;
-        next[u] = i < sp.nvec ? body[i] : V::fill();
-    }
-    for (int base = 0; base < sp.nvec;) {
+    for (int base = lo; base < hi;) {
         uint4 cur[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) cur[u] = next[u];
         base += kU * THREADS;
-        if (base < sp.nvec) {
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int i = base + u * THREADS + tid;
-                next[u] = i < sp.nvec ? body[i] : V::fill();
-            }
-        }
+        if (base < hi) fetch(base);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             float v[V::N];
@@ -1110,9 +1118,25 @@ __device__ __forceinline__ Acc sum_row(const typename Elem<DT>::Raw* x, int voca
     return acc;
 }
 
+// The sums of a row's parts, for few long rows (launch_step): (R, s) of part p of a row at
+// partial[2 * (row * parts + p)].
+template <int DT, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_parts_kernel(const DistillArgs a) {
+    __shared__ Acc lds[THREADS / kWave];
+    const int64_t row = a.row0 + blockIdx.x;
+    const typename Elem<DT>::Raw* x = static_cast<const typename Elem<DT>::Raw*>(a.x) + a.rows.offset(row);
+    const Acc acc = acc_block<false, THREADS>(sum_row<DT, THREADS>(x, a.vocab, a.scale.k, blockIdx.y, gridDim.y), lds);
+    if (threadIdx.x == 0) {
+        float* o = a.partial + 2 * (row * gridDim.y + blockIdx.y);
+        o[0] = acc.R;
+        o[1] = acc.s;
+    }
+}
+
 // LOSS alone: the sums of a row.  GRAD alone: from the sums of an earlier call; a row may be cut in
-// parts (blockIdx.y).  Both: the row is read twice, the second time from the memory-side cache as long
-// as the rows under way fit there (see launch_step).
+// parts (blockIdx.y).  Both, in parts: from the sums of distill_parts_kernel.  Both, whole: the row is
+// read twice, the second time from the memory-side cache as long as the rows under way fit there (see
+// launch_step).
 template <int DT, int THREADS, bool LOSS, bool GRAD, bool LAST>
 __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     using E = Elem<DT>;
@@ -1120,7 +1144,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     __shared__ float red[THREADS / kWave];
     __shared__ TeacherLds l;
     const int64_t row = a.row0 + blockIdx.x;
-    const int part = blockIdx.y, parts = gridDim.y;              // LOSS: one part
+    const int part = blockIdx.y, parts = gridDim.y;              // LOSS alone: one part
     const typename E::Raw* x = static_cast<const typename E::Raw*>(a.x) + a.rows.offset(row);
     const float weight = a.t.row_weight ? a.t.row_weight[row] : 1.0f;
     const float c = GRAD ? weight * a.t.tau * (a.row_grad ? a.row_grad[row] : 1.0f) : 0.0f;
@@ -1136,12 +1160,20 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     bool off = weight == 0.0f;                                   // nothing of the row's logits counts
     if (LOSS) {
         Acc acc = acc_empty();
-        if (!off) acc = sum_row<DT, THREADS>(x, a.vocab, a.scale.k);
-        acc = acc_block<false, THREADS>(acc, lds);
+        if (GRAD && parts > 1) {                                 // every wave joins them all; at most 64
+            const int p = threadIdx.x % kWave;
+            const float* o = a.partial + 2 * (row * parts + (p < parts ? p : 0));
+            if (p < parts) acc = {o[0], o[1], 0.0f};
+            acc = acc_wave<false>(acc);
+            __syncthreads();
+        } else {
+            if (!off) acc = sum_row<DT, THREADS>(x, a.vocab, a.scale.k, 0, 1);
+            acc = acc_block<false, THREADS>(acc, lds);
+        }
         off = off || l.empty;
         st = {acc.R, acc.s, 0.0f, log2f(acc.s), 0.0f, false};
         if (!off && !acc_good(acc)) st = slow_stat<DT, THREADS>(x, a.vocab, a.scale.inv_tau, red);
-        if (first_wave) {
+        if (first_wave && part == 0) {
             const float loss = off ? 0.0f : row_loss(a, e, st, weight, l.bad);
             if (threadIdx.x == 0) {
                 a.loss[row] = loss;
@@ -1172,8 +1204,8 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillArgs a) {
     stores_done();
     if (first_wave) {
         const Span sp = Vec<DT>::span(x, a.vocab);
-        const int lo = part == 0 ? 0 : sp.head + static_cast<int>(static_cast<int64_t>(sp.nvec) * part / parts) * Vec<DT>::N;
-        const int hi = part == parts - 1 ? a.vocab : sp.head + static_cast<int>(static_cast<int64_t>(sp.nvec) * (part + 1) / parts) * Vec<DT>::N;
+        const int lo = part == 0 ? 0 : sp.head + part_of(sp, part, parts).lo * Vec<DT>::N;
+        const int hi = part == parts - 1 ? a.vocab : sp.head + part_of(sp, part, parts).hi * Vec<DT>::N;
         fix_row<DT>(g, l, a.t.k, lo, hi, f);
     }
 }
@@ -1758,6 +1790,17 @@ void launch_step(const fa_logits* x, const DistillArgs& a, hipStream_t st) {
     const int nvec = x->vocab / Vec<DT>::N;
     if (nvec <= kWave * 4) return launch_step_t<DT, 4>(rows, a, st);
     if (nvec <= kWave * 8) return launch_step_t<DT, 8>(rows, a, st);
+    // Few long rows fill the chip only in parts, at the price of a second launch: 1 x 128000 bf16 13.4 us
+    // in parts, 21.7 whole; 128 x 128000 bf16 22.4 and 25.5; 4 x 1000000 fp32 17 and 199.  At 200 KB a
+    // row the GPU gains as much as the launch costs the host (1 x 50261 fp32: 12.0 and 13.8, called one
+    // by one 16.0 and 13.7).  Not where the gradient goes over the logits: a block reads the teacher's
+    // tokens in other parts, whose blocks may have written them.
+    if (a.partial && a.grad != a.x && rows <= FA_DISTILL_WS_ROWS && row_bytes(x) >= FA_DISTILL_WS_BYTES) {
+        int parts = 2;
+        while (parts < kWave && rows * parts * 2 <= FA_DISTILL_WS_FLOATS / 2 && nvec / (parts * 2) >= 1024) parts *= 2;
+        hipLaunchKernelGGL((distill_parts_kernel<DT, 256>), dim3(static_cast<unsigned>(rows), parts), dim3(256), 0, st, a);
+        return launch_distill_t<DT, 256, true, true, false>(rows, parts, a, st);
+    }
     const bool last = rows * row_bytes(x) > kMemoryCache;
     if (wide_blocks(rows, x->vocab) || row_bytes(x) > (128 << 10)) {
         if (last) launch_distill_t<DT, 1024, true, true, true>(rows, 1, a, st);
@@ -1873,15 +1916,16 @@ int fa_distill_grad(const fa_logits* x, const fa_teacher* t, const float* stat, 
 }
 
 int fa_distill_loss_grad(const fa_logits* x, const fa_teacher* t, float* loss, void* grad, int64_t grad_stride_outer,
-                         int64_t grad_stride_inner, fa_stream_t stream) {
+                         int64_t grad_stride_inner, float* ws, fa_stream_t stream) {
     int rc = check_logits(x);
     if (rc == FA_OK) rc = check_teacher(t, x->outer * x->inner);
     if (rc != FA_OK) return rc;
     if (x->outer * x->inner == 0) return FA_OK;
     if (!loss || !grad || grad_stride_outer < 0 || grad_stride_inner < 0) return FA_ERR_INVALID;
-    if (!aligned_to(grad, elem_size(x->dtype))) return FA_ERR_ALIGN;
+    if (!aligned_to(grad, elem_size(x->dtype)) || !aligned_to(ws, sizeof(float))) return FA_ERR_ALIGN;
     DistillArgs a = distill_args(x, t);
     a.loss = loss;
+    a.partial = ws;
     a.grad = grad;
     a.grad_rows = {x->inner, grad_stride_outer, grad_stride_inner};
     switch (x->dtype) {

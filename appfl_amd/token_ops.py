@@ -286,7 +286,10 @@ def distill_loss_grad(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.T
         torch.autograd.graph.increment_version(out)          # a graph that saved it must not use it
         so, si = (0, out.stride(0)) if len(lead) == 1 else out.stride()[:2]
     loss = _new(lead, _f32)
-    rc = N.load().fa_distill_loss_grad(C.byref(x), C.byref(t), loss.data_ptr(), out.data_ptr(), so, si,
+    ws = None
+    if x.outer * x.inner <= N.FA_DISTILL_WS_ROWS and x.vocab * logits.element_size() >= N.FA_DISTILL_WS_BYTES:
+        ws = _new((N.FA_DISTILL_WS_FLOATS,), _f32)
+    rc = N.load().fa_distill_loss_grad(C.byref(x), C.byref(t), loss.data_ptr(), out.data_ptr(), so, si, _ptr(ws),
                                        _raw_stream(index))
     if rc:
         N.check(rc, "fa_distill_loss_grad")

@@ -499,6 +499,9 @@ int fa_synth_fill(float* p, const float* base, size_t n, uint64_t seed, uint64_t
 enum { FA_LOGITS_F32 = 0, FA_LOGITS_BF16 = 1, FA_LOGITS_F16 = 2 };
 #define FA_VOCAB_MAX (1 << 30) /* tokens of a vocabulary                                      */
 #define FA_DISTILL_STAT 4      /* floats per row that fa_distill_loss leaves for the gradient */
+#define FA_DISTILL_WS_ROWS 128     /* fa_distill_loss_grad uses its workspace for calls of at most   */
+#define FA_DISTILL_WS_BYTES 204800 /* this many rows of at least this many bytes                     */
+#define FA_DISTILL_WS_FLOATS 2048  /* size of that workspace                                         */
 #define FA_TOP_MAX 256         /* entries of one list                                         */
 #define FA_SCORES_TOP_MAX 128  /* top entries of one fa_token_scores call                     */
 #define FA_MERGE_CLIENTS 128   /* clients of one fa_merge_tops call                           */
@@ -562,7 +565,8 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
  * fa_distill_loss writes the losses and, for the backward call, `stat` (FA_DISTILL_STAT floats a row);
  * fa_distill_grad writes the gradient of sum_r row_grad[r] * loss[r] (row_grad NULL: 1);
  * fa_distill_loss_grad does both (row_grad 1) and may write the gradient over the logits (same
- * data and strides).  The gradient has the logits' type and row shape, with strides of its own;
+ * data and strides); with a device workspace ws (FA_DISTILL_WS_FLOATS floats, one call's at a time;
+ * NULL: none) few long rows are spread over the GPU.  The gradient has the logits' type and row shape, with strides of its own;
  * its rows must not overlap.  A row with weight 0 or without an entry of probability above 0 has
  * loss and gradient 0 whatever its logits hold; an id >= vocab makes its row's loss and gradient
  * NaN.  A logit of -inf has q = 0 (loss inf where the teacher wants it).  Log probabilities are
@@ -574,7 +578,8 @@ int fa_distill_grad(const fa_logits* logits, const fa_teacher* teacher, const fl
                     const float* row_grad, void* grad, int64_t grad_stride_outer,
                     int64_t grad_stride_inner, fa_stream_t stream);
 int fa_distill_loss_grad(const fa_logits* logits, const fa_teacher* teacher, float* loss, void* grad,
-                         int64_t grad_stride_outer, int64_t grad_stride_inner, fa_stream_t stream);
+                         int64_t grad_stride_outer, int64_t grad_stride_inner, float* ws,
+                         fa_stream_t stream);
 
 /*
  * Host-side packing of one client's state dict into a row of a (pinned) staging slab:

@@ -44,7 +44,7 @@ def test_logits_are_checked_by_every_entry(change, code):
     assert lib.fa_token_scores(C.byref(x), None, 0, 0, None, 256, 256, None, None, None) == code
     assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, 256, None) == code
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 256, 30, 10, None) == code
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None) == code
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None, None) == code
 
 
 @pytest.mark.parametrize("change", [
@@ -55,7 +55,7 @@ def test_teachers_are_checked(change):
     x, t = _logits(), _teacher(**change)
     assert lib.fa_distill_loss(C.byref(x), C.byref(t), 256, 256, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 256, 30, 10, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, None, None) == INVALID
 
 
 def test_outputs_and_null_pointers_are_checked():
@@ -76,10 +76,11 @@ def test_outputs_and_null_pointers_are_checked():
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, None, 30, 10, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 256, -1, 10, None) == INVALID
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), 256, None, 258, 30, 10, None) == ALIGN
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, None, 30, 10, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, 256, 30, 10, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, -10, None) == INVALID
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 257, 30, 10, None) == ALIGN
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, None, 30, 10, None, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, 256, 30, 10, None, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, -10, None, None) == INVALID
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 257, 30, 10, None, None) == ALIGN
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), 256, 256, 30, 10, 258, None) == ALIGN
 
 
 def test_merge_arguments_are_checked():
@@ -106,7 +107,7 @@ def test_empty_calls_do_nothing():
     assert lib.fa_token_scores(C.byref(x), None, 0, 0, None, None, None, None, None, None) == 0
     assert lib.fa_distill_loss(C.byref(x), C.byref(t), None, None, None) == 0
     assert lib.fa_distill_grad(C.byref(x), C.byref(t), None, None, None, 0, 0, None) == 0
-    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, None, 0, 0, None) == 0
+    assert lib.fa_distill_loss_grad(C.byref(x), C.byref(t), None, None, 0, 0, None, None) == 0
     tops = _tops()
     assert lib.fa_merge_tops(C.byref(tops), N.double_array([1.0]), 1, 0, 4, None, None, None) == 0
 

@@ -259,6 +259,31 @@ def test_step_in_place_and_into_out(vocab, dtype):
     assert bool((buf[:, :5] == 77.0).all()) and bool((buf[:, 5 + vocab:] == 77.0).all())
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab", [(1, 102401), (2, 700003), (7, 131072), (128, 102407), (129, 102407)])
+def test_step_of_few_long_rows(rows, vocab, dtype):
+    """Rows cut in parts, and one row more than that takes."""
+    x = logits(rows, vocab, dtype, seed=13)
+    ids, lp = teacher(rows, vocab, 9, seed=14)
+    ids[0, :4] = torch.tensor([0, vocab - 1, vocab // 2, 0])          # the ends, and one twice
+    weight = torch.rand(rows) + 0.5
+    if rows > 6:
+        weight[1] = 0.0
+        ids[2, 0] = vocab                                            # outside: NaN
+        x[3, vocab // 3] = math.nan
+        ids[4] = -1                                                  # no entry
+        x[5] = -math.inf
+        x[6, ::2] = -math.inf
+    want_loss, want_grad, loss_tol, grad_tol = R.distill(x, ids, lp, 1.5, weight, None)
+    dev = x.cuda()
+    big = torch.full((rows, vocab + 3), 7.0, dtype=x.dtype, device="cuda")
+    for out in (None, big[:, 1:1 + vocab], big[:, :vocab], dev):      # aligned unlike the logits, and in place
+        loss, grad = ops().distill_loss_grad(dev, ids.cuda(), lp.cuda(), 1.5, weight.cuda(), out=out)
+        R.close(loss, want_loss, loss_tol, "loss")
+        R.close(grad, want_grad, grad_tol, "grad")
+    assert bool((big[:, vocab + 1:] == 7).all())
+
+
 def test_distill_gradient_against_differences():
     rows, vocab, k = 3, 13, 5
     x = logits(rows, vocab, "f32", seed=16, scale=1.0)
