@@ -147,7 +147,10 @@ def run(state):
         case = state["case"]
         if op == "scores":
             s = token_ops.token_scores(state["logits"], state["targets"], top=case["top"])
-            return [s.logprob, s.entropy, s.lse, s.top_ids, s.top_logprobs]
+            lists = [s.top_ids, s.top_logprobs]
+            if case["top"] == 0:                                 # no lists; the plain form's are empty
+                lists = [s.lse.new_empty((*s.lse.shape, 0), dtype=t) for t in (torch.int32, torch.float32)]
+            return [s.logprob, s.entropy, s.lse, *lists]
         if op == "merge":
             return list(token_ops.merge_tops(state["ids"], state["logprobs"], state["weights"], case["top"],
                                              token_weight=state["token_weight"]))
