@@ -518,7 +518,7 @@ def test_results_do_not_change_from_call_to_call():
         assert torch.equal(merged[0], m2[0]) and torch.equal(merged[1], m2[1])
 
 
-@pytest.mark.parametrize("rows,vocab", [(2, 40009), (64, 1009)])
+@pytest.mark.parametrize("rows,vocab", [(2, 40009), (64, 1009), (3, 110017)])
 def test_captured_and_replayed(rows, vocab):
     """The whole path in one graph, replayed on new inputs with eager work in between."""
     o = ops()
@@ -562,6 +562,24 @@ def test_two_streams_at_once():
     for i in range(2):
         for s in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(s[1:], want[i][1:]))
+
+
+def test_steps_in_parts_on_two_streams_at_once():
+    o = ops()
+    x = [logits(3, 120011, "bf16", seed=70 + i).cuda() for i in range(2)]
+    ids, lp = [t.cuda() for t in teacher(3, 120011, 8, seed=72)]
+    want = [o.distill_loss_grad(v, ids, lp) for v in x]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(o.distill_loss_grad(x[i], ids, lp))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
 
 
 def test_refusals():
