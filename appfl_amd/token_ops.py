@@ -230,18 +230,16 @@ class _Distill(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, row_grad):
         # Python costs three times as much in autograd's threads: the forward call's structures are used
-        # again, with pointers (and, if they changed, strides) anew, because hooks on saved tensors may
-        # hand back other memory than was saved.
+        # again, unless hooks on saved tensors handed back other memory than was saved.  They are never
+        # written to: another backward pass of the graph may be under way.
         logits, stat, ids, logprobs, row_weight = ctx.saved_tensors
         x, t, strides, id_stride, lp_stride = ctx.call
-        if logits.stride() != strides or ids.stride(0) != id_stride or logprobs.stride(0) != lp_stride:
+        if (logits.data_ptr() != (x.data or 0) or ids.data_ptr() != (t.ids or 0) or
+                logprobs.data_ptr() != (t.logprobs or 0) or (_ptr(row_weight) or 0) != (t.row_weight or 0) or
+                logits.stride() != strides or ids.stride(0) != id_stride or logprobs.stride(0) != lp_stride):
             x = _logits(logits)
-            t = N.Teacher(None, None, ids.stride(0), logprobs.stride(0), None, t.temperature, t.k)
-        else:
-            x.data = logits.data_ptr()
-        t.ids, t.logprobs = ids.data_ptr(), logprobs.data_ptr()
-        if row_weight is not None:
-            t.row_weight = row_weight.data_ptr()
+            t = N.Teacher(ids.data_ptr(), logprobs.data_ptr(), ids.stride(0), logprobs.stride(0), _ptr(row_weight),
+                          t.temperature, t.k)
         if not row_grad.is_contiguous():
             row_grad = row_grad.contiguous()
         grad = _new(logits.shape, logits.dtype)

@@ -461,6 +461,27 @@ def test_hooks_on_saved_tensors():
     R.close(grad, want, tol, "grad")
 
 
+def test_backward_leaves_the_forward_call_as_it_was():
+    """A second backward pass of the same graph may be under way in another thread."""
+    x = logits(3, 50, "f32", seed=80).cuda().requires_grad_(True)
+    ids, lp = teacher(3, 50, 4, seed=81)
+    weight = torch.rand(3).cuda()
+    held = []
+
+    def elsewhere(t):
+        held.append(t.clone())
+        return held[-1]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, elsewhere):
+        loss = ops().distill_loss(x, ids.cuda(), lp.cuda(), row_weight=weight)
+    call = loss.grad_fn.call[:2]
+    before = [bytes(c) for c in call]
+    grads = [torch.autograd.grad(loss.sum(), x, retain_graph=True)[0] for _ in range(2)]
+    assert [bytes(c) for c in call] == before
+    _, want, _, tol = R.distill(x.detach().cpu(), ids, lp, 1.0, weight.cpu())
+    for g in grads:
+        R.close(g, want, tol, "grad")
+
+
 def test_a_step_over_saved_logits_is_noticed():
     """The gradient written over logits that an earlier loss saved: that loss's backward pass must refuse."""
     x = torch.randn(3, 17, device="cuda")
