@@ -156,9 +156,13 @@ __device__ __forceinline__ void store_once(uint4* p, const uint4& r) {
 //   s = sum 2^(x k - R),   e = sum 2^(x k - R) (x k - R)   (entropy = (log2 s - e / s) / k)
 // R is raised only when a value passes it by more than 2^kSlack: terms are then at most that large,
 // which fp32 does not mind.
-// R stays within +-kFar, so a distance is finite; a row whose x k lies beyond (a row of the type's
-// lowest value, infinities) or holds a NaN ends with s = 0, inf or NaN and is taken again by
-// slow_stat, which subtracts the maximum before it scales.
+// R stays within +-kFar, so a distance is finite.  From |x k| = 2^24 on R is a multiple of 2 and more:
+// where all of a lane's values (or of a row's) lie that far out, behind a mask of -1e10 or on a row of
+// padding, its terms are 2^r, r up to half of R's step, and s or e may be inf.  Beside an ordinary
+// value such a lane's sums are dropped (acc_raise).  A row that keeps them holds |r| <= 64 below
+// |x k| = 2^31 (x = 1.5e9 at T = 1); a sum outside 2^+-80, a row beyond +-kFar (the type's lowest value,
+// infinities) and a NaN make acc_good refuse, and the row is taken again by slow_stat, which subtracts
+// the maximum before it scales.
 constexpr float kFar = 1e38f;
 
 struct Acc {
@@ -170,11 +174,14 @@ __device__ __forceinline__ Acc acc_empty() { return {-kFar, 0.0f, 0.0f}; }
 // exp2 of the hardware: below 2^-126 it returns 0, which is nothing beside the largest term
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
+// Sums below 2^-126 of the new reference are dropped whole: scaled, an infinite one would be a NaN.  A
+// NaN stays; a lane with a logit of +inf holds R = kFar, above which nothing is raised.
 template <bool ENT>
 __device__ __forceinline__ void acc_raise(Acc& a, float R) {
     const float d = a.R - R, f = exp2_hw(d);
-    if (ENT) a.e = f * (a.e + a.s * d);
-    a.s *= f;
+    const bool gone = f == 0.0f && a.s == a.s;
+    if (ENT) a.e = gone ? 0.0f : f * (a.e + a.s * d);
+    a.s = gone ? 0.0f : a.s * f;
     a.R = R;
 }
 
@@ -199,10 +206,11 @@ __device__ __forceinline__ void acc_add(Acc& a, const float (&v)[N], float top, 
 
 template <bool ENT>
 __device__ __forceinline__ Acc acc_join(Acc a, Acc b) {
-    const float R = fmaxf(a.R, b.R);
-    acc_raise<ENT>(a, R);
-    acc_raise<ENT>(b, R);
-    return {R, a.s + b.s, a.e + b.e};
+    const bool up = a.R >= b.R;                    // never NaN
+    const Acc hi = up ? a : b;
+    Acc lo = up ? b : a;
+    acc_raise<ENT>(lo, hi.R);
+    return {hi.R, hi.s + lo.s, hi.e + lo.e};
 }
 
 template <bool ENT>
@@ -291,7 +299,8 @@ __device__ __attribute__((noinline)) RowStat slow_stat(const typename Elem<DT>::
     return r;
 }
 
-__device__ __forceinline__ bool acc_good(const Acc& a) { return a.s > 0.0f && a.s < kInf; }
+// Within 2^+-80 s, its reciprocal and a gradient's factor over it keep all of their bits.
+__device__ __forceinline__ bool acc_good(const Acc& a) { return a.s > 0x1p-80f && a.s < 0x1p80f && fabsf(a.e) < kInf; }
 
 struct Scale {               // k = fl(log2(e) / T), 1 / k, 1 / T
     float k, inv_k, inv_tau;

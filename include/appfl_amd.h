@@ -537,9 +537,11 @@ typedef struct {             /* entry j of client c's row r at ids[c * id_client
  *   logprob = x_target - lse (0 where target == ignore_index, NaN where it is outside the
  *   vocabulary);  top_ids / top_logprobs: the `top` largest logits, best first, equal ones (and -0
  *   and +0) by the lower id first, NaN before everything.
- * A row of nothing but -inf has lse = -inf, entropy 0 and log probabilities of -inf.  Sums are fp32:
- * near 0 the entropy's and the log probabilities' errors are absolute, some 1e-7.  targets and
- * logprob may both be NULL; 0 <= top <= min(vocab, FA_SCORES_TOP_MAX).
+ * A row of nothing but -inf has lse = -inf, entropy 0 and log probabilities of -inf; one with a NaN or
+ * +inf has NaN for all of them.  Sums are fp32: near 0 the entropy's and the log probabilities' errors
+ * are absolute, some 1e-7 (1e-5 in a row whose largest logit lies beyond +-1e7, as one does that is
+ * masked throughout by a finite value).  targets and logprob may both be NULL;
+ * 0 <= top <= min(vocab, FA_SCORES_TOP_MAX).
  */
 int fa_token_scores(const fa_logits* logits, const int64_t* targets, int64_t ignore_index, int top,
                     float* logprob, float* entropy, float* lse, int32_t* top_ids,

@@ -660,3 +660,59 @@ def test_refusals():
     buf = torch.zeros(6, 9, device="cuda")
     with pytest.raises(ValueError):
         o.distill_loss_grad(buf[:3], ids, lp, out=buf[2:5])
+
+
+# ---- finite masks ------------------------------------------------------------------------------------
+
+MASKS = {"f32": [-1e9, -2.5e9, -1e10, -1e18, -1e30], "bf16": [-1e9, -1.66e9, -2.5e9, -1e10, -1e30], "f16": [-1e4, -6e4]}
+PLACES = ["front", "back", "groups", "all but one"]
+
+
+def finite_masks(rows, vocab, dtype, seed, keep=None):
+    """Ordinary logits, of which every row masks a run, whole lanes' elements or all but one, by another finite value;
+    the elements `keep` [rows, k] stay."""
+    x = logits(rows, vocab, dtype, seed=seed)
+    i = torch.arange(vocab)
+    for r in range(rows):
+        place = PLACES[r // len(MASKS[dtype]) % len(PLACES)]
+        out = {"front": i < vocab // 2, "back": i >= vocab // 2, "groups": i // 64 % 2 == 0, "all but one": i != vocab // 3}[place]
+        if keep is not None:
+            out = out.scatter(0, keep[r].long(), False)
+        x[r, out] = MASKS[dtype][r % len(MASKS[dtype])]
+    return x
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab,top", [(20, 1024, 8), (20, 1023, 64), (20, 20011, 128), (520, 5003, 128), (520, 5003, 0)])
+def test_scores_behind_finite_masks(rows, vocab, top, dtype):
+    check_scores(finite_masks(rows, vocab, dtype, seed=90), some_targets(rows, vocab), top)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab", [(20, 1024), (20, 5003), (20, 110017), (20, 70001)])
+def test_distill_behind_finite_masks(rows, vocab, dtype):
+    """The mask beside the teacher's tokens, and over some of them."""
+    ids, lp = teacher(rows, vocab, 6, seed=91)
+    for keep in (ids, None):
+        for tau in (1.0, 0.5, 4.0):
+            check_distill(finite_masks(rows, vocab, dtype, seed=92, keep=keep), ids, lp, tau)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab", [(6, 1000), (6, 20011), (520, 5003)])
+def test_scores_of_rows_masked_throughout(rows, vocab, dtype):
+    """Every element the same finite value: all tokens alike.
+
+    x log2(e) below 2^31 is at most 64 away from the whole number beside it, so a row's terms are 2^r, |r| <= 64: log2 s
+    (below 2^7 here) rounds by 2^-18, e / s by r times what a sum is off (a rounding of 2^-24 each of vocab / 64 + 64
+    additions, one multiply-add a term) and 2^-18 more; in natural units all of it times ln 2 < 1."""
+    for mask in MASKS[dtype]:
+        x = torch.full((rows, vocab), mask).to(DTYPES[dtype])
+        s = ops().token_scores(x.cuda(), torch.arange(rows).cuda() % vocab, top=min(vocab, 128))
+        even = math.log(vocab)
+        tol = 2.0 ** -16 + (64 + 1) * (vocab / 64 + 66) * 2.0 ** -24
+        for name, want in (("entropy", even), ("logprob", -even), ("top_logprobs", -even)):
+            assert float((getattr(s, name).double() - want).abs().max()) <= tol, (mask, name)
+        want = float(x[0, 0]) + even
+        assert float((s.lse.double() - want).abs().max()) <= 2.0 ** -22 * abs(want) + tol, mask
+        assert torch.equal(s.top_ids.cpu(), torch.arange(min(vocab, 128), dtype=torch.int32).expand(rows, -1))
