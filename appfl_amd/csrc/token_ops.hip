@@ -803,7 +803,7 @@ __global__ __launch_bounds__(THREADS, scores_waves(THREADS, TOP)) void token_sco
     if (!acc_good(acc)) {
         st = slow_stat<DT, THREADS>(x, a.vocab, a.scale.inv_tau, red);
         lse = st.m + st.log_s;
-        fits = false;
+        fits = fits && st.s == st.s;         // lists do not depend on the sums, but the comparisons above pass a NaN by
     }
     if (TOP && !fits) slow_top<DT, THREADS>(x, a.vocab, a.top, l);
     if (tid == 0) {

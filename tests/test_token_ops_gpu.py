@@ -716,3 +716,22 @@ def test_scores_of_rows_masked_throughout(rows, vocab, dtype):
         want = float(x[0, 0]) + even
         assert float((s.lse.double() - want).abs().max()) <= 2.0 ** -22 * abs(want) + tol, mask
         assert torch.equal(s.top_ids.cpu(), torch.arange(min(vocab, 128), dtype=torch.int32).expand(rows, -1))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab,top", [(6, 1000, 64), (6, 1000, 128), (6, 20011, 128), (520, 9001, 128), (520, 9001, 5)])
+def test_lists_of_padding_rows(rows, vocab, top, dtype):
+    """Rows whose sums are taken a second time (nothing but -inf, the type's lowest or largest value) among rows whose
+    lists have to be as well (NaN, +inf) and ordinary ones, over several chunks and with long lists."""
+    x = logits(rows, vocab, dtype, seed=93)
+    x[0] = -math.inf
+    x[1] = torch.finfo(x.dtype).min
+    x[2, ::3] = torch.finfo(x.dtype).max
+    x[3, 1::2] = -math.inf
+    x[3, ::2] = torch.finfo(x.dtype).min
+    x[4, vocab - 2] = math.nan
+    check_scores(x, some_targets(rows, vocab), top)
+    x[5, vocab - 3] = math.inf
+    x[5, 7] = math.inf
+    s = ops().token_scores(x.cuda(), top=top)
+    assert s.top_ids[5, :2].tolist() == [7, vocab - 3]
