@@ -1308,9 +1308,11 @@ __global__ __launch_bounds__(THREADS) void distill_step_kernel(const DistillArgs
 // ---- merging the clients' lists -------------------------------------------------------------------
 // One block per row, every entry in a register of its thread.  Entries are grouped by a hash table in
 // LDS.  A group's probabilities are added as whole numbers, scaled by the power of two that puts the
-// group's largest below 2^51: at most 2^13 entries stay below 2^64, whole numbers add up to the same
-// sum in any order, and a sum is off by no more than 2^-51 of the largest term per entry (fp64
-// additions: 2^-53 of the sum each).  The groups' values are then ranked, ties to the lowest id.
+// group's largest below 2^51: whole numbers add up to the same sum in any order, and a sum is off by
+// no more than 2^-51 of the largest term per entry (fp64 additions: 2^-53 of the sum each).  A term
+// may be rounded up to 2^51, and 2^13 of those are 2^64: that sum alone comes out as 0, which a
+// group's is not otherwise, its largest term being 2^50 at least (or subnormal).  The groups' values
+// are then ranked, ties to the lowest id.
 // A table takes kFull different tokens, and those that are on their way when it fills; a row with more
 // is merged in rounds, each of which takes the tokens that got into the table and ranks them together
 // with the best of the rounds before.
@@ -1399,7 +1401,7 @@ __device__ __forceinline__ unsigned exponent_of(double p) { return static_cast<u
 constexpr int merge_waves(int threads, int per) { return per >= 8 ? 4 : threads == 256 ? (per == 4 ? 5 : 8) : 6; }
 
 // e^v of an fp32 value in fp64: 2^n times the Taylor series of e^r, |r| <= ln 2 / 2, whose first
-// omitted term is below 2^-57; log2(e) in two parts keeps r exact to fp64.  About half the
+// omitted term is below 2^-57; ln 2 in two parts keeps r exact to fp64.  About half the
 // instructions of the library's, which has to take any fp64 argument.
 __device__ __forceinline__ double exp_of(float v) {
     const double x = static_cast<double>(fminf(fmaxf(v, -1000.0f), 1000.0f));       // beyond: 0 and inf; NaN see below
@@ -1571,8 +1573,9 @@ __global__ __launch_bounds__(THREADS, merge_waves(THREADS, PER)) void merge_tops
                 const unsigned x = l.peak[s];
                 const uint64_t sum = l.sum[s];
                 name[e] = l.token[s];
+                const double whole = x && !sum ? 0x1p64 : static_cast<double>(sum);
                 const double v = x == kExpInf ? (sum >> 32 ? __builtin_nan("") : __builtin_inf())
-                                              : ldexp(static_cast<double>(sum), static_cast<int>(x ? x : 1) - 1022 - 51);
+                                              : ldexp(whole, static_cast<int>(x ? x : 1) - 1022 - 51);
                 key[e] = v != v ? 0x7ff8000000000000ull : static_cast<uint64_t>(__double_as_longlong(v));
             }
         }

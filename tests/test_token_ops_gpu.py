@@ -735,3 +735,14 @@ def test_lists_of_padding_rows(rows, vocab, top, dtype):
     x[5, 7] = math.inf
     s = ops().token_scores(x.cuda(), top=top)
     assert s.top_ids[5, :2].tolist() == [7, vocab - 3]
+
+
+def test_merge_of_the_most_entries_of_one_token():
+    """Every entry of every list the same token, its terms the largest below a power of two."""
+    K, k = 32, 256
+    ids = torch.full((K, 2, k), 5, dtype=torch.int32)
+    ids[:, 1, 0] = 9                                # 8160 of them, and another token
+    lp = torch.zeros(K, 2, k)
+    weights = [1.0 - 2.0 ** -53] * K
+    check_merge(ids, lp, weights, 3)
+    check_merge(ids, lp, weights, 3, torch.ones(K, 2))
