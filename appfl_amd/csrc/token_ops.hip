@@ -1977,7 +1977,16 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
     a.per_k = ((1ull << 32) + in->k - 1) / in->k;
     a.out_ids = out_ids;
     a.out_lp = out_logprobs;
-    for (int c = 0; c < K; ++c) a.w[c] = w[c];
+    // Only the weights' ratios count: by a power of two (exact) the largest is put into [1/2, 1), so that
+    // products and sums stay within fp64.  A weight that is nothing beside it still answers.
+    double most = 0.0;
+    for (int c = 0; c < K; ++c) most = w[c] > most ? w[c] : most;
+    int power = 0;
+    frexp(most, &power);
+    for (int c = 0; c < K; ++c) {
+        a.w[c] = ldexp(w[c], -power);
+        if (w[c] > 0.0 && a.w[c] == 0.0) a.w[c] = 4.9406564584124654e-324;
+    }
     return launch_merge(a, rows, as_stream(stream));
 }
 

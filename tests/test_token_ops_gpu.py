@@ -746,3 +746,26 @@ def test_merge_of_the_most_entries_of_one_token():
     weights = [1.0 - 2.0 ** -53] * K
     check_merge(ids, lp, weights, 3)
     check_merge(ids, lp, weights, 3, torch.ones(K, 2))
+
+
+@pytest.mark.parametrize("power", [1023, 900, -900, -1070])
+def test_merge_with_weights_at_the_ends_of_their_type(power):
+    """Only the weights' ratios count: the same bits at any power of two, up to fp64's largest and down to its least."""
+    K, rows, k = 3, 5, 7
+    ids, lp = answers(K, rows, k, 20, seed=8)
+    unit = torch.rand(K, rows) + 0.5
+    base = [1.5, 1.25, 1.75]
+    check_merge(ids, lp, base, 9, unit)
+    want = ops().merge_tops(ids.cuda(), lp.cuda(), base, 9, token_weight=unit.cuda())
+    got = ops().merge_tops(ids.cuda(), lp.cuda(), [math.ldexp(b, power) for b in base], 9, token_weight=unit.cuda())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_merge_with_weights_of_all_sizes():
+    """A client whose weight is nothing beside another's still answers: its tokens come behind."""
+    ids = torch.tensor([[[3, 4]], [[5, 4]]], dtype=torch.int32)
+    lp = torch.log(torch.tensor([[[0.5, 0.25]], [[0.5, 0.25]]]))
+    got_ids, got_lp = ops().merge_tops(ids.cuda(), lp.cuda(), [1e308, 5e-324], 4)
+    assert got_ids.cpu().tolist() == [[3, 4, 5, -1]]
+    R.close(got_lp[0, :2], lp[0, 0].double(), 2.0 ** -24 * 2 + 1e-11)
+    assert float(got_lp[0, 2]) < -700.0
