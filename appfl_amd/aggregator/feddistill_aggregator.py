@@ -16,6 +16,7 @@ counterpart among the reference's aggregators.
 
 from __future__ import annotations
 
+import math
 from typing import Any, Dict, List, Optional, Tuple
 
 import torch
@@ -28,8 +29,8 @@ class FedDistillAggregator(BaseAggregator, DeviceStateMixin):
     """
     :param `model`: optional model; `get_parameters` hands out its state before the first round.
     :param `aggregator_configs`: `client_weights_mode` ("equal" or "sample_size"), `top` (entries of
-        the teacher's lists; default: as many as the longest client list), `temperature` (of `loss`,
-        default 1.0), `device`.
+        the teacher's lists, with absent ones behind where a round brings fewer; default: as many as
+        the longest client list), `temperature` (of `loss`, default 1.0), `device`.
     :param `logger`: optional logger.
     """
 
@@ -60,7 +61,12 @@ class FedDistillAggregator(BaseAggregator, DeviceStateMixin):
                 raise ValueError("no client answers to aggregate")
             ids, logprobs, unit = self._stack(local_models)
             top = int(self.top) if self.top is not None else ids.shape[2]
-            self.teacher = token_ops.merge_tops(ids, logprobs, self._weights(local_models), top, token_weight=unit)
+            most = ids.shape[0] * ids.shape[2]                   # entries a row can have; behind them absent ones
+            merged = token_ops.merge_tops(ids, logprobs, self._weights(local_models),
+                                          top if top > token_ops.TOP_MAX else min(top, most), token_weight=unit)
+            if top > most:
+                merged = tuple(torch.nn.functional.pad(t, (0, top - most), value=v) for t, v in zip(merged, (-1, -math.inf)))
+            self.teacher = merged
             return self._download()
 
     def answer(self, logits: torch.Tensor, targets: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:

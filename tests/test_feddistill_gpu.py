@@ -131,3 +131,30 @@ def test_registration():
     cls = plugin.register_distillation(m)["FedDistillAggregator"]
     assert m.FedDistillAggregator is cls and issubclass(cls, BaseAggregator)
     assert cls(None, {"top": 2}, None).top == 2
+
+
+@pytest.mark.parametrize("sizes,top", [((3,), 8), ((2, 3, 1), 16), ((4, 4), 256)])
+def test_more_entries_asked_for_than_clients_send(sizes, top):
+    """`top` above what the clients of a round list together: the lists end with absent entries."""
+    vocab, rows = 31, 4
+    agg = aggregator(top=top, temperature=2.0)
+    updates, ids, lps = {}, [], []
+    longest = max(sizes)
+    for c, k in enumerate(sizes):
+        g = torch.Generator().manual_seed(c)
+        i = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(rows)]).int()
+        v = torch.log_softmax(torch.randn(rows, k + 1, generator=g), 1)[:, :k]
+        updates[f"c{c}"] = {"top_ids": i, "top_logprobs": v}
+        ids.append(torch.nn.functional.pad(i, (0, longest - k), value=-1))
+        lps.append(torch.nn.functional.pad(v, (0, longest - k), value=-math.inf))
+    got = agg.aggregate(updates)
+    want_ids, want_lp = R.merge(torch.stack(ids), torch.stack(lps), [1.0 / len(sizes)] * len(sizes), top)
+    assert got["top_ids"].shape == (rows, top) and torch.equal(got["top_ids"], want_ids)
+    R.close(got["top_logprobs"], want_lp, 2.0 ** -24 * want_lp.abs().nan_to_num(posinf=0.0) + 1e-11)
+    assert bool((got["top_ids"][:, sum(sizes):] == -1).all())
+    x = torch.randn(rows, vocab, generator=torch.Generator().manual_seed(9))
+    want_loss, want_grad, loss_tol, grad_tol = R.distill(x, got["top_ids"], got["top_logprobs"], 2.0)
+    loss, grad = agg.loss_grad(x.cuda())
+    assert bool(loss.isfinite().all())
+    R.close(loss, want_loss, loss_tol, "loss")
+    R.close(grad, want_grad, grad_tol, "grad")
