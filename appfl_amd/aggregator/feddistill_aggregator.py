@@ -115,7 +115,8 @@ class FedDistillAggregator(BaseAggregator, DeviceStateMixin):
         if not 0 <= first <= first + rows <= ids.shape[0]:
             raise ValueError(f"positions {first}..{first + rows} of a teacher of {ids.shape[0]}")
         part = slice(first, first + rows)
-        return ids[part].view(lead + (-1,)), logprobs[part].view(lead + (-1,))
+        shape = lead + (ids.shape[1],)
+        return ids[part].view(shape), logprobs[part].view(shape)
 
     def _weights(self, local_models: Dict) -> List[float]:
         sizes = getattr(self, "client_sample_size", None) or {}

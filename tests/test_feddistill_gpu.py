@@ -158,3 +158,15 @@ def test_more_entries_asked_for_than_clients_send(sizes, top):
     assert bool(loss.isfinite().all())
     R.close(loss, want_loss, loss_tol, "loss")
     R.close(grad, want_grad, grad_tol, "grad")
+
+
+def test_losses_of_no_rows():
+    agg = aggregator(top=2)
+    agg.aggregate({"a": {"top_ids": torch.zeros(4, 2, dtype=torch.int32), "top_logprobs": torch.zeros(4, 2)}})
+    for shape in ((0, 5), (2, 0, 5), (0, 3, 5)):
+        x = torch.zeros(shape, device="cuda", requires_grad=True)
+        loss = agg.loss(x, first=4)
+        loss.sum().backward()
+        assert loss.shape == shape[:-1] and x.grad.shape == shape
+        loss, grad = agg.loss_grad(x.detach())
+        assert loss.shape == shape[:-1] and grad.shape == shape
