@@ -72,10 +72,14 @@ class FedDistillAggregator(BaseAggregator, DeviceStateMixin):
     def answer(self, logits: torch.Tensor, targets: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
         """A client's update from its model's logits (``[rows, vocab]`` or ``[batch, rows, vocab]`` on
         the GPU), as tensors of that GPU with one row per position, with the `entropy` of every
-        position and, if `targets` are given, their `logprob`."""
+        position and, if `targets` are given, their `logprob`.  The lists hold `top` entries, or
+        as many as there are tokens (classes), and at most 128."""
         if self.top is None:
             raise ValueError("answer needs the configuration's `top`")
-        s = token_ops.token_scores(logits, targets, top=int(self.top))
+        top = min(int(self.top), token_ops.SCORES_TOP_MAX)
+        if isinstance(logits, torch.Tensor) and logits.dim():
+            top = min(top, logits.shape[-1])
+        s = token_ops.token_scores(logits, targets, top=top)
         out = {"top_ids": s.top_ids.flatten(0, -2), "top_logprobs": s.top_logprobs.flatten(0, -2),
                "entropy": s.entropy.flatten()}
         if targets is not None:

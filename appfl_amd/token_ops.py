@@ -25,7 +25,7 @@ import torch
 from . import _native as N
 
 DTYPES = {torch.float32: N.FA_LOGITS_F32, torch.bfloat16: N.FA_LOGITS_BF16, torch.float16: N.FA_LOGITS_F16}
-TOP_MAX = N.FA_TOP_MAX
+TOP_MAX, SCORES_TOP_MAX = N.FA_TOP_MAX, N.FA_SCORES_TOP_MAX
 
 # The smallest calls take less time on the GPU than in Python, so the checks below look at each
 # property once, the stream's handle is read without making a Stream object, and results are

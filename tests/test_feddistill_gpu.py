@@ -170,3 +170,15 @@ def test_losses_of_no_rows():
         assert loss.shape == shape[:-1] and x.grad.shape == shape
         loss, grad = agg.loss_grad(x.detach())
         assert loss.shape == shape[:-1] and grad.shape == shape
+
+
+@pytest.mark.parametrize("classes,top", [(10, 32), (10, 10), (1, 5), (300, 200)])
+def test_answers_of_fewer_classes_than_entries(classes, top):
+    """`top` above the classes there are, or above one call's lists: an answer holds what there is."""
+    agg = aggregator(top=top)
+    x = torch.randn(6, classes, generator=torch.Generator().manual_seed(3))
+    a = agg.answer(x.cuda())
+    n = min(classes, top, 128)
+    want, tol = R.scores(x, None, n)
+    assert torch.equal(a["top_ids"].cpu(), want["top_ids"])
+    R.close(a["top_logprobs"], want["top_logprobs"], tol["top_logprobs"])
