@@ -29,10 +29,17 @@ TOP_MAX, SCORES_TOP_MAX = N.FA_TOP_MAX, N.FA_SCORES_TOP_MAX
 
 # The smallest calls take less time on the GPU than in Python, so the checks below look at each
 # property once, the stream's handle is read without making a Stream object, and results are
-# allocated without the dispatcher (0.7 instead of 1.4-1.9 us each) where torch has that call.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# allocated without the dispatcher (0.7 instead of 1.4-1.9 us each) where torch has those calls.  A
+# torch that was built without a GPU lacks them, and imports this module all the same.
 _f32, _i32, _i64 = torch.float32, torch.int32, torch.int64
+
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current_device
+except ImportError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+    _current_device = torch.cuda.current_device
 
 try:
     from torch._C._dynamo.guards import _empty_strided_cuda as _empty_strided

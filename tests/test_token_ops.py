@@ -141,3 +141,21 @@ def test_reference_agrees_with_torch():
     kl.sum().backward()
     loss, grad, _, _ = R.distill(x, ids, lp, 2.0)
     assert torch.allclose(loss, kl.detach()) and torch.allclose(grad, leaf.grad)
+
+
+def test_the_package_imports_without_a_gpu_build_of_torch():
+    """Such a build lacks the calls that read the current stream and device; host tensors are refused as ever."""
+    import os
+    import subprocess
+    import sys
+
+    code = ("import torch\n"
+            "for name in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+            "import appfl_amd, appfl_amd.aggregator\n"
+            "from appfl_amd import _native, token_ops\n"
+            "try: token_ops.token_scores(torch.zeros(2, 5))\n"
+            "except _native.NativeLibraryError: print('refused')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0 and done.stdout.strip() == "refused", done.stderr
