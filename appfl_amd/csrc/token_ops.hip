@@ -971,22 +971,28 @@ __device__ __forceinline__ void teacher_unite(int k, TeacherLds& l) {
     }
 }
 
-// The loss, by the first wave.
+// The loss, by the first wave.  Where the teacher wants what a mask has taken out, log q is x / T to all its
+// bits; T^2 t x / T is then added as T (t x / 4) * 4, since x / T, and the sum of all t x, may be beyond fp32.
 __device__ __forceinline__ float row_loss(const DistillArgs& a, const Teacher& e, const RowStat& st, float weight, bool bad) {
-    float sum = 0.0f;
+    float sum = 0.0f, far = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         if (!(e.t[i] > 0.0f)) continue;
-        float log_q;
+        const bool none = e.x[i] == -kInf;
+        float log_q, apart;
         if (st.slow) {
-            log_q = e.x[i] == -kInf ? -kInf : (e.x[i] - st.m) * a.scale.inv_tau - st.log_s;
+            apart = none ? -kInf : 0.25f * e.x[i] - 0.25f * st.m;
+            log_q = none ? -kInf : (e.x[i] - st.m) * a.scale.inv_tau - st.log_s;
         } else {
             const float y = fmaf(e.x[i], a.scale.k, -st.R) - st.log_s;
-            log_q = fabsf(y) < 1e30f ? y * kLn2 : e.x[i] * a.scale.inv_tau;
+            apart = 0.25f * e.x[i];
+            log_q = y * kLn2;
         }
-        sum += e.t[i] * (e.log_t[i] - log_q);
+        if (log_q < -1e30f) far -= e.t[i] * apart;
+        else sum += e.t[i] * (e.log_t[i] - log_q);
     }
     sum = wave_sum_f(sum) * (a.t.tau * a.t.tau) * weight;
+    if (__any(far != 0.0f)) sum += wave_sum_f(far) * (a.t.tau * weight) * 4.0f;
     return bad || st.s != st.s ? __builtin_nanf("") : sum;
 }
 

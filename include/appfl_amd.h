@@ -573,7 +573,7 @@ int fa_merge_tops(const fa_tops* in, const double* w, int K, int64_t rows, int t
  * its rows must not overlap.  A row with weight 0 or without an entry of probability above 0 has
  * loss and gradient 0 whatever its logits hold; an id >= vocab makes its row's loss and gradient
  * NaN.  A logit of -inf has q = 0 (loss inf where the teacher wants it).  Log probabilities are
- * fp32, off by some 2^-20: the loss by T^2 times that.
+ * fp32, off by some 2^-20: the loss by T^2 times that.  An entry with t below 2^-126 counts as absent.
  */
 int fa_distill_loss(const fa_logits* logits, const fa_teacher* teacher, float* loss, float* stat,
                     fa_stream_t stream);

@@ -769,3 +769,25 @@ def test_merge_with_weights_of_all_sizes():
     assert got_ids.cpu().tolist() == [[3, 4, 5, -1]]
     R.close(got_lp[0, :2], lp[0, 0].double(), 2.0 ** -24 * 2 + 1e-11)
     assert float(got_lp[0, 2]) < -700.0
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+# The lists' least t is 3e-20 at T = 1/4 (below 2^-126 an entry is none); T * 3.4e38 fits fp32 up to 1.
+@pytest.mark.parametrize("tau", [0.25, 0.5, 1.0])
+@pytest.mark.parametrize("vocab", [40, 5003, 110017])
+def test_distill_with_the_lowest_value_under_the_teacher(vocab, tau, dtype):
+    """T^2 t (m - x) / T is finite where x / T is not; beside -inf it is inf."""
+    rows, k = 6, 5
+    x = logits(rows, vocab, dtype, seed=94)
+    ids, lp = teacher(rows, vocab, k, seed=95)
+    low = torch.finfo(x.dtype).min
+    x[0, int(ids[0, 1])] = low
+    x[1, ids[1].long()] = low
+    x[2] = low
+    x[2, int(ids[2, 0])] = 1.0
+    x[3, ids[3].long()] = low
+    x[3, int(ids[3, 0])] = -math.inf                # the best entry
+    x[4] = -math.inf
+    x[4, :2] = low
+    weight = torch.tensor([1.0, 0.25, -1.0, 1.0, 1.0, 0.5])
+    check_distill(x, ids, lp, tau, weight)
