@@ -904,17 +904,19 @@ __device__ __forceinline__ void teacher_gather(const typename Elem<DT>::Raw* x, 
 
 __device__ __forceinline__ void teacher_make(Teacher& r, int vocab, float inv_tau, TeacherLds& l) {
     const int lane = threadIdx.x;
-    bool bad = false;
+    bool outside = false, broken = false;
     float peak = -kInf;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         if (r.id[i] < 0) r.lp[i] = -kInf;
-        bad = bad || r.id[i] >= vocab || r.lp[i] != r.lp[i] || r.lp[i] == kInf;
+        outside = outside || r.id[i] >= vocab;
+        broken = broken || r.lp[i] != r.lp[i];
         peak = fmaxf(peak, r.lp[i]);
     }
-    bad = __any(bad);
+    broken = __any(broken);
     peak = wave_max_f(peak);
-    const bool empty = !bad && peak == -kInf;
+    const bool empty = !broken && peak == -kInf;                 // whatever its ids
+    const bool bad = broken || __any(outside) || peak == kInf;
     float z = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {

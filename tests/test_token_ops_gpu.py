@@ -791,3 +791,17 @@ def test_distill_with_the_lowest_value_under_the_teacher(vocab, tau, dtype):
     x[4, :2] = low
     weight = torch.tensor([1.0, 0.25, -1.0, 1.0, 1.0, 0.5])
     check_distill(x, ids, lp, tau, weight)
+
+
+@pytest.mark.parametrize("vocab", [40, 5003, 110017])
+def test_distill_rows_without_an_entry_whatever_their_ids(vocab):
+    """Nothing of probability above 0: loss and gradient 0, also where an id is outside the vocabulary; NaN shows."""
+    rows, k = 5, 3
+    x = logits(rows, vocab, "f32", seed=96)
+    ids, lp = teacher(rows, vocab, k, seed=97)
+    ids[0], lp[0] = vocab + 5, -math.inf
+    ids[1], lp[1] = torch.tensor([-1, vocab, 2]), torch.tensor([0.5, -math.inf, -math.inf])
+    ids[2, 1], lp[2, 1] = vocab, -math.inf           # beside entries that count: NaN
+    lp[3] = math.nan
+    x[0] = math.nan
+    check_distill(x, ids, lp, 1.0)
