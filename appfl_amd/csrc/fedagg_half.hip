@@ -989,6 +989,11 @@ int late_mode() {
 // than bfloat16, its tile-per-block kernel being a little faster -- two-moment optimizers 25.6 M x
 // 48 / 64 / 100 -4.2 / -4.1 / -7.4 %, 47 M x 64 -8.5 %, 8-17 M x 64 -0.8...-4.2 %, but 17 M x 48 +4 %;
 // FedAvgM 25.6 M x 48 / 64 -3.3 / -5.3 %, 47 M x 32 -3.8 %; plain FedAvg 8-87 M x 48-64 -3.4...-5.9 %.
+// These figures are from a build with packed fp32 instructions.  Without them, 4.5-162 M elements x 8-100
+// clients x plain FedAvg, FedAvgM and FedAdam: the shapes this rule gives to the late-epilogue kernel
+// -2.9 % on average in bfloat16 and -2.7 % in float16 (25.6 M x 64 FedAdam -9.2 and -6.1 %), the others from
+// 8 M up +12 and +6 %.  A shape moves by up to 10 % with where its rows lie (17 M x 64 FedAdam +6.2 and
+// -3.5 %), so that the borders stand as they are.
 bool late_wins(int half, int opt, int K, double tiles) {
     if (half != FA_HALF_BF16) {
         if (opt == FA_OPT_NONE) return (K >= 48 && tiles >= 3.5) || (K >= 32 && tiles >= 22.0);

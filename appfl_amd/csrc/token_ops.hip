@@ -5,8 +5,10 @@
 //
 // Softmax sums are fp32 (below), lists are ranked by whole keys, merged probabilities are fp64 terms
 // added as 64-bit whole numbers (their order decides which tokens are kept).  Nothing is rounded to 16
-// bits but a gradient's elements, once.  A block takes a row; blocks share nothing, there is no
-// workspace, and no float is added atomically, so results are the same in every run.
+// bits but a gradient's elements, once.  A block takes a row, and few long rows of a gradient, or of loss
+// and gradient in one call, are cut in parts (launch_grad, launch_step; the latter with a workspace of the
+// call's own).  Blocks of one launch share nothing and no float is added atomically, so results are the
+// same in every run.
 //
 // What bounds them (one MI355X): scores and the gradient alone move 5.0-6.9 TB/s of their bytes (8192 x
 // 128000 bf16: lists of 8 351 us, sums alone 322; a gradient 855 us), loss and gradient in one call

@@ -127,7 +127,8 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, t
     """Scores of every row of `logits` (fa_token_scores): ``lse = log sum_v exp x_v``, the entropy
     of ``softmax(x)`` in nats, the log probability of ``targets`` (int64, the shape of the rows; 0
     where it is `ignore_index`, NaN where it is outside the vocabulary) and the `top` most probable
-    tokens, best first (ties to the lower id), with their log probabilities."""
+    tokens, best first (ties to the lower id), with their log probabilities.  The results carry no
+    gradient, also of logits that require one."""
     x = _logits(logits)
     index = logits.get_device()
     if _current_device() != index:           # launches go to the current device
@@ -263,7 +264,10 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
     fa_distill_grad).  The teacher's list (`ids` int32, `logprobs` float32 log probabilities or
     logits, ``[rows..., k]``) is made a distribution of its own, ``t = softmax(logprobs / T)``, and
     ``loss = row_weight * T**2 * sum_j t_j (log t_j - log softmax(x / T)[ids_j])``.  Rows of weight 0
-    or without an entry have loss and gradient 0; an id outside the vocabulary makes its row NaN."""
+    or without an entry have loss and gradient 0; an id outside the vocabulary makes its row NaN.
+    Only `logits` get a gradient: `logprobs` and `row_weight` are taken as constants, also where they
+    require one.  The log probabilities are fp32, off by some ``2**-20``, the loss by ``T**2`` times
+    that: 2e-5 at ``T = 4``, but 1e-2 at 100 and 1 at 1000."""
     if isinstance(logits, torch.Tensor) and logits.is_cuda and _current_device() != logits.get_device():
         with torch.cuda.device(logits.get_device()):
             return _Distill.apply(logits, ids, logprobs, temperature, row_weight)
